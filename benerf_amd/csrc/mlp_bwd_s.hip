@@ -533,7 +533,7 @@ __global__ __launch_bounds__(BNT, 2) void mlp_bwd_split_kernel(BwdArgs a) {
     const int64_t Mp = m_pad(M);
     uint8_t* st8 = reinterpret_cast<uint8_t*>(dacts + sdact_lo8_base(Mp));      // lo8 region: byte i <-> half i of the SH region
     // ReLU sign-bit words.  h0..h7 (round 5, mlp_split.h): uint32 [layer][tile 128][row tile 4][column tile 8][32], written by the
-    // forward's scalar stores; this lane's feature ct * 32 + (lane & 31) is word sp_mask_word(lane & 31) of block (rt, ct), and the
+    // forward's epilogue; this lane's feature ct * 32 + (lane & 31) is word sp_mask_word(lane & 31) of block (rt, ct), and the
     // 16 points of its accumulator elements are bits 8 (e >> 2) + 4 (lane >> 5) + (e & 3): shifted down by 4 (lane >> 5) once.
     // hv (mask layer 8) keeps the uint64 [64-point tile][4 x 64 threads] format of mlp_common.h (P1 below).
     const __amdgpu_buffer_rsrc_t mask_rsrc =

@@ -12,12 +12,12 @@
 // Range: |x| must stay below 65504 (f16 max) - NeRF activations are O(1..100); every launch folds max|activation|
 // into the caller's status word once it passes 2^15 (mlp_split.h, 'Range guard'), so a violation is never silent.
 // Training mode saves the activations for the backward kernels: BENERF_MLP_SPLIT (SAVE == 2) - f16 hi halves + 8-bit residual codes
-// straight from the epilogue's registers in the SP layout, sign bits through the scalar path (DirectSave below; the narrow hv / PE
+// straight from the epilogue's registers in the SP layout, sign bits as compare masks (DirectSave below; the narrow hv / PE
 // arrays as SH arrays from the finished planes); BENERF_MLP_SPLIT_F16BWD (SAVE == 1) - the hi halves as SH arrays (mlp_split.h).
 #define BENERF_HSW_V2      // this kernel's planes use the round-5 slot swizzle (mlp_split.h: hsw)
 #include "mlp_split.h"
 #if defined(__HIP_DEVICE_COMPILE__) && !defined(__gfx950__)
-#error "mlp_fwd_h.hip is written for gfx950: scalar stores (s_store_dwordx2 + s_dcache_wb), aux = 2 cache policy, v_permlane32_swap"
+#error "mlp_fwd_h.hip is written for gfx950: aux = 2 cache policy, v_permlane32_swap"
 #endif
 // Cache policy of the saved-operand stores (aux of raw_buffer_store on gfx950: 0 default, 1 = sc0, 2 = nt, 16 = sc1).  The activations are
 // written once and read ~2 ms later by another kernel - 2.8 GB per 522 k-point launch streaming through the 4 MiB L2 of an XCD, where the
@@ -58,6 +58,9 @@ struct FwdArgs {
 };
 
 typedef _Float16 half2v __attribute__((ext_vector_type(2)));
+// v_writelane_b32: `old` with lane `at` replaced by the wave-uniform `value`.  The compiler's intrinsic, not inline asm: a mask that a
+// compare has just left in an SGPR pair needs wait states before another vector instruction reads it, which the compiler inserts
+extern "C" __device__ uint32_t write_lane(uint32_t value, uint32_t at, uint32_t old) __asm("llvm.amdgcn.writelane.i32");
 typedef float float2v __attribute__((ext_vector_type(2)));
 typedef short short4v __attribute__((ext_vector_type(4)));
 typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
@@ -101,11 +104,12 @@ __device__ __forceinline__ void acc_init_bias(f32x16 (&acc1)[NR][NCT], const flo
 
 // BENERF_MLP_SPLIT training launches (SAVE == 2, round 5): the stage's activations leave for HBM straight from the epilogue's
 // registers - what a lane holds after the lane exchange IS a 16-byte unit of the SP layout (mlp_split.h: 8 features of one
-// point), hi and scaled lo side by side for the residual codes - and the ReLU sign bits go out through the scalar path
-// (v_cmp_gt_f32 -> SGPR pair -> s_store_dwordx2).  No transpose reads of the finished planes, no per-pair address arithmetic.
+// point), hi and scaled lo side by side for the residual codes - and the ReLU sign bits are compare masks: v_cmp_gt_f32 leaves the
+// 64-lane mask of an accumulator register in an SGPR pair, v_writelane puts its two words into the lanes that store them.  No
+// transpose reads of the finished planes, no per-pair address arithmetic.
 struct DirectSave {
     __amdgpu_buffer_rsrc_t rs, rs8;   // this tile's part of the layer's SP array (hi halves) / of its lo8 twin
-    const uint32_t* mask;             // wave-uniform: sign-bit word ((T * 4 + 0) * 8 + ct) * 32 of the layer, or null (no ReLU)
+    uint32_t* mask;                   // wave-uniform: sign-bit word ((T * 4 + 0) * 8 + ct) * 32 of the layer, or null (no ReLU)
 };
 
 // combine the two accumulators (+ReLU) -> both LDS planes (hi, scaled lo) [-> HBM: sv].
@@ -122,6 +126,7 @@ __device__ __forceinline__ void epilogue_t(f32x16 (&acc1)[NR][NCT], f32x16 (&acc
     // byte offset of this lane's unit (16-point chunk pl >> 4 of the tile, slot 4 ct + hf, point pl & 15) in the tile's part of the SP
     // array; slot + 2 i is an immediate of the store (i * 512), row tile r two chunks (r * 16 384; the lo8 twin: half of everything)
     const int vo = SV ? (((pl >> 4) * 32 + ct0 * 4 + hf) * 16 + (pl & 15)) * 16 : 0;
+    uint32_t bits = 0;        // sign-bit words of two row tiles: lanes 0-31 the even one's 32 words, lanes 32-63 the odd one's
 #pragma unroll
     for (int r = 0; r < NR; ++r) {
         const int row = r * 32 + pl, sw = hsw(row);
@@ -149,14 +154,13 @@ __device__ __forceinline__ void epilogue_t(f32x16 (&acc1)[NR][NCT], f32x16 (&acc
                     }
                     // range guard: amax = max(amax, |v0|, |v1|) as ONE v_max3_f32 (the compiler's IEEE-mode fmaxf chain is two or three)
                     asm("v_max3_f32 %0, %0, |%1|, |%2|" : "+v"(amax) : "v"(v[0]), "v"(v[1]));
-                    if (SV && RELU) {     // sign bits of accumulator elements e, e + 1: 64-lane masks, 8 bytes each, through the scalar cache
+                    if (SV && RELU) {     // sign bits of accumulator elements e, e + 1: 64-lane masks, two words each
 #pragma unroll
                         for (int t = 0; t < 2; ++t) {
-                            uint64_t m;
-                            asm volatile("v_cmp_gt_f32_e64 %0, %1, 0" : "=s"(m) : "v"(v[t]));
-#ifndef FWD_NO_MASK_STORE     /* timing variant (dX then reads stale masks): what do the scalar stores cost? */
-                            asm volatile("s_store_dwordx2 %0, %1, %2" ::"s"(m), "s"(sv->mask), "n"((r * 8 * 32 + 2 * (e + t)) * 4) : "memory");
-#endif
+                            const uint64_t m = __builtin_amdgcn_fcmpf(v[t], 0.f, 2 /* ordered greater */);
+                            const int at = (r & 1) * 32 + 2 * (e + t);
+                            bits = write_lane((uint32_t)m, at, bits);
+                            bits = write_lane((uint32_t)(m >> 32), at + 1, bits);
                         }
                     }
                     const half2v hi = __builtin_convertvector(v, half2v);
@@ -191,6 +195,8 @@ __device__ __forceinline__ void epilogue_t(f32x16 (&acc1)[NR][NCT], f32x16 (&acc
                 }
             }
         }
+        // two row tiles' words in one store: 128 bytes each, 1 KiB apart
+        if (SV && RELU && (r & 1)) __builtin_nontemporal_store(bits, sv->mask + ((r - 1) * 8 * 32 + hf * 8 * 32 + pl));
     }
 }
 
@@ -383,7 +389,7 @@ __global__ __launch_bounds__(FNT, 1) void mlp_fwd_split_kernel(FwdArgs a) {
         DirectSave d;
         d.rs = uniform_rsrc(SAVE == 2 ? st_h + ((int64_t)layer * Mp + ms0) * 256 : nullptr);
         d.rs8 = uniform_rsrc(SAVE == 2 ? st8_h + ((int64_t)layer * Mp + ms0) * 256 : nullptr);
-        d.mask = (SAVE == 2 && relu) ? reinterpret_cast<const uint32_t*>(acts + sact_mask(Mp)) + (int64_t)layer * mask_stride +
+        d.mask = (SAVE == 2 && relu) ? reinterpret_cast<uint32_t*>(acts + sact_mask(Mp)) + (int64_t)layer * mask_stride +
                                            ((int64_t)blockIdx.x * 32 + wave) * 32
                                      : nullptr;
         return d;
@@ -656,9 +662,6 @@ __global__ __launch_bounds__(FNT, 1) void mlp_fwd_split_kernel(FwdArgs a) {
         }
     }
     TRF(20);
-    // the sign-bit words went through the scalar data cache: scalar stores are invisible to the compiler's wait-count tracking, so
-    // wait for them explicitly, then write the cache back
-    if (SAVE == 2) asm volatile("s_waitcnt lgkmcnt(0)\n\ts_dcache_wb" ::: "memory");
 }
 
 }  // namespace

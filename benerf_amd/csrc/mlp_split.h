@@ -227,7 +227,7 @@ __host__ __device__ inline int64_t sp_half_index(int64_t m, int W, int w) {
     return (((m >> 4) * (W >> 3) + (w >> 3)) * 16 + (m & 15)) * 8 + (w & 7);
 }
 // ReLU sign bits of h0..h7 in BENERF_MLP_SPLIT, round 5: straight out of v_cmp_gt_f32 on the forward's accumulators (one VALU
-// instruction per accumulator register -> a 64-lane mask in an SGPR pair -> s_store_dwordx2; tools/hwprobe/sstore_mask.hip).
+// instruction per accumulator register -> a 64-lane mask in an SGPR pair -> two v_writelane into the register that is stored).
 // Accumulator element e of (row tile r, column tile ct) in the transposed product: lanes 0-31 = points 32 r + lane of feature
 // 32 ct + 8 (e >> 2) + (e & 3), lanes 32-63 = the same points of feature + 4.  uint32 word index inside layer l (same region,
 // same stride as before: sact_mask + l * (Mp / 64) * 512 words):   ((T * 4 + r) * 8 + ct) * 32 + 2 e + h,   bit p = point
