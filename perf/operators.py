@@ -179,8 +179,8 @@ def prepare(case, seed):
         lists = dict(exp_avg=views("m"), exp_avg_sq=views("v" if case["bits"] == 32 else "u"), exp_avg_scale=views("ms", BLOCK),
                      exp_avg_sq_scale=views("us", BLOCK), master=views("master"))
         if case["op"] == "adamw":
-            d["grads"] = kernels.GradList(g)
             d["plan"] = kernels.AdamWPlan(views("p"), **lists)
+            d["grads"] = kernels.GradList(g, d["plan"])
             return d
         params = [torch.nn.Parameter(p) for p in views("p")]
         opt = optim.FusedAdamW(params, lr=LR, betas=(BETA1, BETA2), eps=EPS, weight_decay=DECAY, state_bits=case["bits"], max_norm=MAX_NORM,
