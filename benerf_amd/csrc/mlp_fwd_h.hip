@@ -141,13 +141,8 @@ __device__ __forceinline__ void epilogue_t(f32x16 (&acc1)[NR][NCT], f32x16 (&acc
 #pragma unroll
                 for (int jp = 0; jp < 2; ++jp) {
                     const int e = q * 4 + jp * 2;
-                    // v = acc1 + acc2 * 2^-11 for the pair as ONE v_pk_fma_f32 (accumulator registers e, e + 1 are an aligned pair)
-                    float2v v;
-                    {
-                        const float2v a1 = {acc1[r][c][e], acc1[r][c][e + 1]}, a2 = {acc2[r][c][e], acc2[r][c][e + 1]};
-                        const float2v sc = {LO_INV, LO_INV};
-                        asm("v_pk_fma_f32 %0, %1, %2, %3" : "=v"(v) : "v"(a2), "v"(sc), "v"(a1));
-                    }
+                    // v = acc1 + acc2 * 2^-11
+                    float2v v = {__builtin_fmaf(acc2[r][c][e], LO_INV, acc1[r][c][e]), __builtin_fmaf(acc2[r][c][e + 1], LO_INV, acc1[r][c][e + 1])};
                     if (RELU) {     // asm: fmaxf() on an asm result costs a canonicalising v_max_f32 v, v, v in front of the real one
                         asm("v_max_f32 %0, 0, %0" : "+v"(v[0]));
                         asm("v_max_f32 %0, 0, %0" : "+v"(v[1]));
@@ -165,8 +160,8 @@ __device__ __forceinline__ void epilogue_t(f32x16 (&acc1)[NR][NCT], f32x16 (&acc
                     }
                     const half2v hi = __builtin_convertvector(v, half2v);
                     // lo = rn16((v - hi) * 2^11) = rn16(fma(-hi, 2^11, v * 2^11)): every step exact in f32 except the final rounding,
-                    // i.e. the same bits as "convert back, subtract, scale, convert" in three instructions per pair instead of five
-                    // (v_pk_mul_f32, v_fma_mixlo_f16, v_fma_mixhi_f16: hi is read as f16 by the mixed-precision FMA)
+                    // i.e. the same bits as "convert back, subtract, scale, convert" in fewer instructions (two v_mul_f32, v_fma_mixlo_f16,
+                    // v_fma_mixhi_f16: hi is read as f16 by the mixed-precision FMA)
                     const float2v vs = v * LO_SCALE;
                     uint32_t l;
                     asm("v_fma_mixlo_f16 %0, -%1, %4, %2 op_sel_hi:[1,0,0]\n\tv_fma_mixhi_f16 %0, -%1, %4, %3 op_sel:[1,0,0] op_sel_hi:[1,0,0]"
