@@ -34,8 +34,18 @@ class LossCfg(Structure):
                 ("event_threshold", c_float), ("event_coeff", c_float), ("rgb_coeff", c_float)]
 
 
+class AdamwTensor(Structure):
+    _fields_ = [("param", c_void_p), ("exp_avg", c_void_p), ("exp_avg_sq", c_void_p), ("exp_avg_scale", c_void_p), ("exp_avg_sq_scale", c_void_p),
+                ("master", c_void_p), ("n", c_int64), ("first_block", c_int64)]
+
+
+class AdamwCfg(Structure):
+    _fields_ = [("lr", c_double), ("beta1", c_double), ("beta2", c_double), ("eps", c_double), ("weight_decay", c_double), ("grad_scale", c_double),
+                ("step", c_int64), ("seed", c_uint64), ("lr_dev", c_void_p), ("step_dev", c_void_p)]
+
+
 P = c_void_p
-ABI_VERSION = 103       # include/benerf_hip.h: BENERF_ABI_VERSION
+ABI_VERSION = 104       # include/benerf_hip.h: BENERF_ABI_VERSION
 _SIGNATURES = {
     "benerf_version": (c_int, []),
     "benerf_last_error": (c_char_p, []),
@@ -87,6 +97,13 @@ _SIGNATURES = {
     "benerf_gather_rows": (c_int, [P, P, c_int64, c_int, P, P]),
     "benerf_sample_pixels": (c_int, [c_int64, c_int64, ctypes.c_uint64, ctypes.c_uint64, P, P]),
     "benerf_adam_step": (c_int, [P, P, P, P, c_int64, c_double, c_double, c_double, c_double, c_int, c_double, P, P]),
+    "benerf_adamw_plan_bytes": (c_size_t, [P, c_int]),
+    "benerf_adamw_plan_fill": (c_int, [P, c_int, c_int, c_int, P, c_size_t]),
+    "benerf_adamw_step": (c_int, [P, P, P, c_int, POINTER(AdamwCfg), P, P, P]),
+    "benerf_adamw_count": (c_int, [P, P, P, P]),
+    "benerf_grad_norm_partials": (c_size_t, [P]),
+    "benerf_grad_norm_partial": (c_int, [P, P, P, c_int, P, c_size_t, POINTER(c_int64), P]),
+    "benerf_grad_norm_finish": (c_int, [P, c_int64, c_double, c_double, P, c_int, P, P, c_int, P]),
 }
 
 EXPORTED_SYMBOLS = tuple(sorted(_SIGNATURES))

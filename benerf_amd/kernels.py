@@ -685,6 +685,282 @@ def adam_step(param, grad, exp_avg, exp_avg_sq, lr, step, beta1=0.9, beta2=0.999
     params_changed()
 
 
+# ----------------------------------------------------------------------------- K9 optimiser over lists of tensors
+ADAMW_BLOCK = 128                   # consecutive elements that share one scale of an 8-bit moment
+_ELEMENT_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+CODE_TYPE = torch.float8_e4m3fn     # 8-bit moments: a code is an e4m3 number, its value the number times its block's scale
+
+
+def _on(device):
+    """Context that makes `device` the current one (launches go to ITS current stream); free of charge where it already is."""
+    return _NOTHING if _cur_device is not None and device.index == _cur_device() else torch.cuda.device(device)
+
+
+class _Nothing:
+    def __enter__(self):
+        return None
+
+    def __exit__(self, *exc):
+        return False
+
+
+_NOTHING = _Nothing()
+
+
+def _list_tensor(t, name, device, dtypes, numel=None):
+    """Checks one tensor of a list and returns an alias of it that keeps its memory alive whatever the caller does to `t`."""
+    if not torch.is_tensor(t):
+        raise TypeError("%s must be a tensor, got %s" % (name, type(t).__name__))
+    if t.layout is not torch.strided:
+        raise TypeError("%s must be dense, got %s" % (name, t.layout))
+    if not t.is_cuda:
+        raise _lib.BenerfHipError("%s must live on the GPU (got %s); there is no CPU path" % (name, t.device))
+    if device is not None and t.device != device:
+        raise ValueError("%s lives on %s, the list on %s" % (name, t.device, device))
+    if t.dtype not in dtypes:
+        raise TypeError("%s must be %s, got %s" % (name, " or ".join(str(d) for d in dtypes), t.dtype))
+    if not t.is_contiguous():
+        raise ValueError("%s must be contiguous" % name)
+    if numel is not None and t.numel() != numel:
+        raise ValueError("%s must have %d elements, got %d" % (name, numel, t.numel()))
+    return t.detach()
+
+
+class _Part:
+    """The tensors of one element type in a list, and their plan: the host copy and the one on the device."""
+
+    def __init__(self, index, rows, param_type, state_bits, device):
+        lib = _lib.load()
+        n = len(rows)
+        self.index, self.count = index, n              # places in the list
+        table = (_lib.AdamwTensor * n)(*rows)
+        size = lib.benerf_adamw_plan_bytes(table, n)
+        if size == 0:
+            raise ValueError("a tensor of the list is too large")
+        self.host = ctypes.create_string_buffer(size)
+        _lib.check(lib.benerf_adamw_plan_fill(table, n, param_type, state_bits, self.host, size), "adamw_plan_fill")
+        self.state_bits = state_bits
+        with _on(device):
+            # a blocking copy: the plan is there before anything is queued on any stream
+            self.dev = torch.frombuffer(bytearray(self.host.raw), dtype=torch.uint8).to(device)
+            self.stream = _stream()
+            self.partials = int(lib.benerf_grad_norm_partials(self.host))
+
+    def on_device(self):
+        """Address of the device copy for a launch on the current stream."""
+        if _stream() != self.stream:
+            self.dev.record_stream(torch.cuda.current_stream(self.dev.device))
+        return self.dev.data_ptr()
+
+
+class GradList:
+    """Gradients of a list of tensors, checked once and kept alive: float32, bfloat16 or float16, contiguous, on one device; None where
+    there is no gradient.  Use it for gradients that stay where they are (accumulated in place, captured); the operators also take a
+    plain list, which they check at every call.  plan: the AdamWPlan the gradients belong to, or None."""
+
+    def __init__(self, tensors, plan=None):
+        tensors = list(tensors)
+        if plan is not None and len(tensors) != len(plan.numels):
+            raise ValueError("%d gradients for %d tensors" % (len(tensors), len(plan.numels)))
+        self.device = plan.device if plan is not None else next((t.device for t in tensors if torch.is_tensor(t)), None)
+        if self.device is None:
+            raise ValueError("GradList: no gradient in the list")
+        self.tensors = [None if t is None else
+                        _list_tensor(t, "gradient %d" % k, self.device, tuple(_ELEMENT_TYPES), None if plan is None else plan.numels[k])
+                        for k, t in enumerate(tensors)]
+        if plan is not None:
+            self.parts = plan.parts
+        else:
+            self.parts = [_Part(range(len(tensors)), [_lib.AdamwTensor(n=0 if t is None else t.numel()) for t in self.tensors], 0, 0, self.device)]
+        self.launches = _grad_launches(self.parts, self.tensors)
+
+    @classmethod
+    def of_checked(cls, tensors, plan):
+        """The gradients of a plan's own parameters (contiguous; torch holds their sizes and devices to the parameters'): no checks."""
+        self = cls.__new__(cls)
+        self.device, self.tensors, self.parts = plan.device, tensors, plan.parts
+        self.launches = _grad_launches(plan.parts, tensors)
+        return self
+
+
+def _grad_launches(parts, tensors):
+    """[(part, element type, array of device addresses)]: one launch sequence for every type of gradient in every part."""
+    out = []
+    for part in parts:
+        by_type = {}
+        for k, i in enumerate(part.index):
+            t = tensors[i]
+            if t is not None:
+                a = by_type.get(t.dtype)
+                if a is None:
+                    a = by_type[t.dtype] = (ctypes.c_void_p * part.count)()
+                a[k] = t.data_ptr()
+        out += [(part, _ELEMENT_TYPES[d], a) for d, a in by_type.items()]
+    return out
+
+
+def _no_overlap(lists):
+    """Refuses tensors that share memory: two workgroups would write the same elements."""
+    spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for l in lists if l is not None for t in l if t is not None and t.numel())
+    if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
+        raise ValueError("two tensors of the list share memory (the same tensor twice?)")
+
+
+class AdamWPlan:
+    """A list of parameters with their moments, ready for `adamw_step` (K9, include/benerf_hip.h: benerf_adamw_plan_fill).
+
+    params: float32, bfloat16 or float16 tensors, contiguous, on one device (types may be mixed).  exp_avg, exp_avg_sq: either float32
+    tensors of the same sizes (moments in 32 bits), or float8_e4m3fn ones together with exp_avg_scale, exp_avg_sq_scale, float32 with
+    ceil(n / 128) elements each (moments in 8 bits; exp_avg_sq then holds the codes of the ROOT of the second moment).  master: None, or
+    float32 copies of the parameters that are bfloat16 / float16 (None at the float32 ones): the step reads and updates those and rounds
+    them into the parameters.  All tensors are updated where they are; the plan keeps them alive and must be made again when a parameter
+    moves.  Making one copies a table to the device and waits for it: not inside a captured region."""
+
+    def __init__(self, params, exp_avg, exp_avg_sq, exp_avg_scale=None, exp_avg_sq_scale=None, master=None):
+        params = list(params)
+        n = len(params)
+        if n == 0:
+            raise ValueError("AdamWPlan: empty list")
+        if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
+            raise _lib.BenerfHipError("AdamWPlan: make the plan before the capture")
+        self.device = params[0].device if torch.is_tensor(params[0]) else None
+        self.params = [_list_tensor(p, "parameter %d" % k, self.device, tuple(_ELEMENT_TYPES)) for k, p in enumerate(params)]
+        self.numels = [p.numel() for p in self.params]
+
+        def like(ts, name, dtype, blocks=False):
+            ts = list(ts)
+            if len(ts) != n:
+                raise ValueError("%s: %d tensors for %d parameters" % (name, len(ts), n))
+            return [_list_tensor(t, "%s %d" % (name, k), self.device, (dtype,), -(-self.numels[k] // ADAMW_BLOCK) if blocks else self.numels[k])
+                    for k, t in enumerate(ts)]
+        exp_avg, exp_avg_sq = list(exp_avg), list(exp_avg_sq)
+        self.state_bits = 8 if exp_avg and torch.is_tensor(exp_avg[0]) and exp_avg[0].dtype == CODE_TYPE else 32
+        if (self.state_bits == 8) != (exp_avg_scale is not None) or (self.state_bits == 8) != (exp_avg_sq_scale is not None):
+            raise ValueError("AdamWPlan: 8-bit moments (float8_e4m3fn) come with exp_avg_scale and exp_avg_sq_scale, 32-bit moments without")
+        kind = CODE_TYPE if self.state_bits == 8 else torch.float32
+        self.exp_avg, self.exp_avg_sq = like(exp_avg, "exp_avg", kind), like(exp_avg_sq, "exp_avg_sq", kind)
+        self.exp_avg_scale = self.exp_avg_sq_scale = None
+        if self.state_bits == 8:
+            self.exp_avg_scale = like(exp_avg_scale, "exp_avg_scale", torch.float32, True)
+            self.exp_avg_sq_scale = like(exp_avg_sq_scale, "exp_avg_sq_scale", torch.float32, True)
+        self.master = None
+        if master is not None:
+            master = list(master)
+            if len(master) != n:
+                raise ValueError("master: %d tensors for %d parameters" % (len(master), n))
+            self.master = []
+            for k, (p, t) in enumerate(zip(self.params, master)):
+                if p.dtype == torch.float32:
+                    if t is not None:
+                        raise ValueError("master %d: a float32 parameter is its own master copy" % k)
+                    self.master.append(None)
+                else:
+                    self.master.append(_list_tensor(t, "master %d" % k, self.device, (torch.float32,), self.numels[k]))
+        mlp_status(self.device)             # the guard's words exist (and are zero) before a step can be captured
+        _no_overlap([self.params, self.exp_avg, self.exp_avg_sq, self.exp_avg_scale, self.exp_avg_sq_scale, self.master])
+        at = lambda l, k: None if l is None or l[k] is None else l[k].data_ptr()       # noqa: E731
+        rows, block = {}, 0
+        for k, p in enumerate(self.params):
+            rows.setdefault(p.dtype, []).append((k, _lib.AdamwTensor(
+                param=p.data_ptr(), exp_avg=at(self.exp_avg, k), exp_avg_sq=at(self.exp_avg_sq, k), exp_avg_scale=at(self.exp_avg_scale, k),
+                exp_avg_sq_scale=at(self.exp_avg_sq_scale, k), master=at(self.master, k), n=p.numel(), first_block=block)))
+            block += -(-p.numel() // ADAMW_BLOCK)
+        self.parts = [_Part([k for k, _ in r], [x for _, x in r], _ELEMENT_TYPES[d], self.state_bits, self.device) for d, r in rows.items()]
+
+
+def _as_grads(grads, plan=None):
+    if not isinstance(grads, GradList):
+        return GradList(grads, plan)
+    if plan is None or grads.parts is plan.parts:
+        return grads
+    if len(grads.tensors) != len(plan.numels) or grads.device != plan.device or \
+            any(g is not None and g.numel() != n for g, n in zip(grads.tensors, plan.numels)):
+        raise ValueError("the gradients do not belong to this plan")
+    return grads
+
+
+def _guard_words(device, guard_range, status):
+    return (mlp_status(device) if status is None else status).data_ptr() if guard_range else None
+
+
+def grad_norm(grads, max_norm=float("inf"), grad_scale=1.0, out=None, counters=(), guard_range=False, status=None):
+    """2-norm over all gradients of a list (GradList, a list of tensors, or a list of GradLists: one norm over all of them), on the
+    device and without synchronising.  Returns float32 [4] = [norm of grad_scale * gradients, coefficient min(1, max_norm / (norm +
+    1e-6)), 1 if the step must be skipped (norm not finite, or guard_range and the range guard's words say so), skipped steps so far];
+    hand it to `adamw_step(norm=...)`.  out: such a tensor (zeroed once by the caller) to write, whose count of skipped steps goes on.
+    counters: float32 1-element step counters on the device that go up by one unless the step is skipped."""
+    lib = _lib.load()
+    if not max_norm > 0:
+        raise ValueError("grad_norm: max_norm must be positive, got %r" % (max_norm,))
+    lists = [grads] if isinstance(grads, GradList) else list(grads)
+    lists = [g if isinstance(g, GradList) else _as_grads(g) for g in (lists if lists and isinstance(lists[0], GradList) else [lists])]
+    dev = lists[0].device
+    if any(g.device != dev for g in lists):
+        raise ValueError("grad_norm: gradients on several devices")
+    launches = [x for g in lists for x in g.launches]
+    with _on(dev):
+        room = sum(part.partials for part, _, _ in launches)
+        partials = torch.empty(max(room, 1), dtype=torch.float64, device=dev)
+        words = torch.empty(4, dtype=torch.float32, device=dev) if out is None else out
+        if out is not None and (_chk(out, name="out") is None or out.numel() != 4 or out.device != dev):
+            raise ValueError("grad_norm: out must have 4 elements on %s" % dev)
+        stream, used, base = _stream(), ctypes.c_int64(), partials.data_ptr()
+        at = 0
+        for part, kind, ptrs in launches:
+            _lib.check(lib.benerf_grad_norm_partial(part.host, part.on_device(), ptrs, kind, base + 8 * at, room - at, ctypes.byref(used), stream),
+                       "grad_norm_partial")
+            at += used.value
+        cs = None
+        if counters:
+            cs = (ctypes.c_void_p * len(counters))(*[_counter(c, dev) for c in counters])
+        _lib.check(lib.benerf_grad_norm_finish(base, at, max_norm, grad_scale, words.data_ptr(), int(out is not None),
+                                               _guard_words(dev, guard_range, status), cs, len(counters), stream), "grad_norm_finish")
+    return words
+
+
+def _counter(t, device):
+    if t.numel() != 1 or t.device != device:
+        raise ValueError("a counter on the device is one float32 on %s" % device)
+    return _chk(t, name="counter")
+
+
+def adamw_count(step, norm=None, guard_range=True, status=None):
+    """One device step counter (float32, 1 element) goes up by one, unless `norm` or the range guard says that the step is skipped."""
+    with _on(step.device):
+        _lib.check(_lib.load().benerf_adamw_count(_counter(step, step.device), _chk(norm, name="norm"), _guard_words(step.device, guard_range, status),
+                                                  _stream()), "adamw_count")
+
+
+def adamw_step(plan, grads, lr, step, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.0, grad_scale=1.0, norm=None, seed=0, guard_range=True, status=None):
+    """One AdamW step over the tensors of an AdamWPlan.  grads: GradList or a list (None: the tensor is left alone).  lr: a number, or
+    one float32 on the device.  step: t of this step from 1, or one float32 on the device that holds it (adamw_count, grad_norm(counters=)
+    count) - needed in a captured step, whose numbers are frozen.  norm: what grad_norm returned - clips, and skips the step where it says
+    so; without a device counter t then counts applied steps.  seed: stochastic rounding of 8-bit moments.  guard_range, status: as in
+    `adam_step`."""
+    lib = _lib.load()
+    grads = _as_grads(grads, plan)
+    cfg = _lib.AdamwCfg(beta1=betas[0], beta2=betas[1], eps=eps, weight_decay=weight_decay, grad_scale=grad_scale, seed=int(seed) & 0xFFFFFFFFFFFFFFFF)
+    dev = plan.device
+    with _on(dev):
+        if torch.is_tensor(step):
+            cfg.step_dev = _counter(step, dev)
+        else:
+            if torch.cuda.is_current_stream_capturing():
+                raise _lib.BenerfHipError("adamw_step: a captured step needs its counter on the device (step=tensor)")
+            cfg.step = int(step)
+        if torch.is_tensor(lr):
+            cfg.lr_dev = _counter(lr, dev)
+        else:
+            cfg.lr = lr
+        if norm is not None and (norm.numel() != 4 or norm.device != dev):
+            raise ValueError("adamw_step: norm must be the 4 words of grad_norm on %s" % dev)
+        words, guard, stream = _chk(norm, name="norm"), _guard_words(dev, guard_range, status), _stream()
+        launches = grads.launches if grads.parts is plan.parts else _grad_launches(plan.parts, grads.tensors)
+        for part, kind, ptrs in launches:
+            _lib.check(lib.benerf_adamw_step(part.host, part.on_device(), ptrs, kind, ctypes.byref(cfg), words, guard, stream), "adamw_step")
+    params_changed()
+
+
 # ----------------------------------------------------------------------------- stand-alone helpers
 def sample_pdf(bins, weights, n_draws, u=None, seed=0, offset=0, want_inds=False):
     lib = _lib.load()

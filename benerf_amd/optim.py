@@ -18,7 +18,12 @@ writes `param_group["lr"]` on them (train.py:196-200, 343-394); checkpoints stor
 
 Arithmetic = torch's Adam with default betas / eps (benerf_adam_step is pinned by golden vector G10).  Options that change the
 update rule (weight_decay, amsgrad, maximize) are refused: the reference never sets them.
+
+`FusedAdamW` is the AdamW next to it (K9): any list of parameters where they live, decoupled decay, clipping by the global norm without
+a synchronisation, moments in 32 or 8 bits, float32 master copies of half-precision parameters.
 """
+import itertools
+
 import torch
 
 from . import kernels as K
@@ -207,3 +212,250 @@ class FlatAdam(torch.optim.Adam):
             o, k, t = run
             K.adam_step(a.p[o:o + k], a.g[o:o + k], a.m[o:o + k], a.v[o:o + k], lr, t, beta1, beta2, eps)
         return None
+
+
+def encode_moment(x):
+    """A float32 moment in 8 bits, to nearest: (float8_e4m3fn codes of x's shape, float32 scale of every 128 consecutive elements).  For
+    a checkpoint of 32-bit moments; the step itself rounds stochastically (include/benerf_hip.h, K9).  Encode the ROOT of exp_avg_sq."""
+    n = x.numel()
+    pad = torch.zeros(-(-n // K.ADAMW_BLOCK) * K.ADAMW_BLOCK, dtype=torch.float32, device=x.device)
+    pad[:n] = x.detach().reshape(-1)
+    rows = pad.view(-1, K.ADAMW_BLOCK)
+    top = torch.where(rows.isfinite(), rows.abs(), 0.0).amax(1)
+    exponent = (torch.frexp(top)[1] - 1).clamp_min(-100) - 7
+    scale = ((exponent.to(torch.int32) + 127) << 23).view(torch.float32)
+    code = torch.where(rows.isfinite(), rows / scale[:, None], float("nan")).view(-1)[:n]
+    return code.to(K.CODE_TYPE).view(x.shape), scale
+
+
+def decode_moment(code, scale):
+    """The float32 values that 8-bit codes and their scales stand for."""
+    return (code.reshape(-1).to(torch.float32) * scale.repeat_interleave(K.ADAMW_BLOCK)[:code.numel()]).view(code.shape)
+
+
+class _Cohort:
+    """Parameters of a group that have made the same steps: one counter (torch's `step`), shared by their state dicts."""
+
+    def __init__(self, step, members):
+        self.step, self.members = step, members
+
+
+class _Group:
+    """What a step needs of one parameter group, made once and again when something moved."""
+
+    def __init__(self, params, plan, states, cohorts):
+        self.params, self.plan, self.states, self.cohorts = params, plan, states, cohorts
+        self.at = [p.data_ptr() for p in params]
+        self.kept = [(st, st["exp_avg"], st["exp_avg_sq"], st["step"]) for st in states]
+
+
+class FusedAdamW(torch.optim.AdamW):
+    """torch.optim.AdamW (decoupled weight decay; same param_groups, state and state_dict) whose step() is one K9 launch per group.
+
+    Parameters stay where they are: float32, bfloat16 or float16, contiguous, on one device.  A parameter without a gradient is left
+    alone, with its moments and its counter; a parameter that has moved (`p.data = ...`) is followed.
+      state_bits  32: exp_avg, exp_avg_sq in float32, whatever the parameter's type.  8: exp_avg in float8_e4m3fn and exp_avg_sq as the
+                  float8_e4m3fn codes of its ROOT, exp_avg_scale and exp_avg_sq_scale with a float32 for every 128 elements, rounded
+                  stochastically with `seed` (16.1 instead of 28 bytes of traffic and 2.1 instead of 8 of memory per parameter).
+                  load_state_dict takes either form (encode_moment / decode_moment).
+      max_norm    None, or the global 2-norm over ALL groups to which gradients are clipped in the same step; a norm that is not finite
+                  skips the step on the device.  After step(), grad_norm holds [norm, coefficient, skipped?, steps skipped so far].
+      master      float32 copies (state["master"]) of half-precision parameters: read and updated instead of them, rounded into them.
+      capturable  counters live on the device, a step can be captured (make one step before, outside; learning rates that change need
+                  `lr` as a float32 tensor on the device).  With max_norm they live there too.
+      guard_range skip the step where the MLP's range guard says so, like FlatAdam.
+    amsgrad, maximize and differentiable are refused."""
+
+    STATE_KEYS = ("exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale", "master")
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, *, state_bits=32, max_norm=None, master=False,
+                 capturable=False, seed=0, guard_range=True, **kw):
+        if state_bits not in (8, 32):
+            raise ValueError("FusedAdamW: moments have 8 or 32 bits, not %r" % (state_bits,))
+        if max_norm is not None and not max_norm > 0:
+            raise ValueError("FusedAdamW: max_norm must be positive, got %r" % (max_norm,))
+        self._settings = dict(state_bits=state_bits, max_norm=max_norm, master=bool(master), seed=int(seed), guard_range=bool(guard_range))
+        self._plans = {}
+        self.grad_norm = None
+        super().__init__(params, lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, capturable=capturable, **kw)
+
+    state_bits = property(lambda self: self._settings["state_bits"])
+    max_norm = property(lambda self: self._settings["max_norm"])
+
+    def __getstate__(self):
+        return dict(super().__getstate__(), _settings=self._settings)
+
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        self._plans = {}
+        self.grad_norm = None
+
+    def load_state_dict(self, state_dict):
+        super().load_state_dict(state_dict)
+        # torch casts state to its parameter's type: moments, codes and master copies keep the one that they were saved in
+        saved = itertools.chain.from_iterable(g["params"] for g in state_dict["param_groups"])
+        mine = itertools.chain.from_iterable(g["params"] for g in self.param_groups)
+        for key, p in zip(saved, mine):
+            st = state_dict["state"].get(key)
+            if st:
+                for name in self.STATE_KEYS:
+                    if torch.is_tensor(st.get(name)):
+                        self.state[p][name] = st[name].detach().to(device=p.device, copy=True)
+        self._plans = {}
+
+    # -- state --------------------------------------------------------------------------------------------------------------
+    def _counts_on_device(self, group):
+        return bool(group.get("capturable")) or self.max_norm is not None
+
+    def _adopt(self, params):
+        """state[p] of every parameter in the form this optimiser keeps: what fits stays where it is, another form is converted, what
+        is missing starts at zero (flat buffers, a tensor's slot at a multiple of 128 elements)."""
+        bits = self.state_bits
+        kind = K.CODE_TYPE if bits == 8 else torch.float32
+        B = K.ADAMW_BLOCK
+        need = {"exp_avg": [], "exp_avg_sq": []}
+        for p in params:
+            st = self.state[p]
+            if bits == 32 and "exp_avg_scale" in st:
+                st["exp_avg"] = decode_moment(st["exp_avg"], st.pop("exp_avg_scale"))
+                st["exp_avg_sq"] = decode_moment(st["exp_avg_sq"], st.pop("exp_avg_sq_scale")).square_()
+            for name, ts in need.items():
+                x = st.get(name)
+                if x is None:
+                    ts.append(p)
+                elif x.numel() != p.numel():
+                    raise ValueError("FusedAdamW: state %s has %d elements, its parameter %d" % (name, x.numel(), p.numel()))
+                elif bits == 8 and name + "_scale" not in st:
+                    x = x.to(device=p.device, dtype=torch.float32)
+                    st[name], st[name + "_scale"] = encode_moment(x.sqrt() if name == "exp_avg_sq" else x)
+                else:
+                    st[name] = x.to(device=p.device, dtype=kind).contiguous()
+                    if bits == 8:
+                        st[name + "_scale"] = st[name + "_scale"].to(device=p.device, dtype=torch.float32).contiguous()
+        for name, ts in need.items():
+            blocks = [-(-p.numel() // B) for p in ts]
+            if not ts:
+                continue
+            flat = torch.zeros(sum(blocks) * B, dtype=torch.uint8 if bits == 8 else torch.float32, device=ts[0].device)
+            flat = flat.view(kind)
+            scale = torch.zeros(sum(blocks), dtype=torch.float32, device=ts[0].device) if bits == 8 else None
+            at = 0
+            for p, b in zip(ts, blocks):
+                self.state[p][name] = flat[at * B:at * B + p.numel()].view(p.shape)
+                if bits == 8:
+                    self.state[p][name + "_scale"] = scale[at:at + b]
+                at += b
+        if self._settings["master"]:
+            for p in params:
+                st = self.state[p]
+                if p.dtype != torch.float32:
+                    x = st.get("master")
+                    st["master"] = p.detach().float() if x is None else x.to(device=p.device, dtype=torch.float32).contiguous()
+
+    def _make(self, group):
+        params = list(group["params"])
+        self._adopt(params)
+        states = [self.state[p] for p in params]
+        scales = {}
+        if self.state_bits == 8:
+            scales = {name: [st[name] for st in states] for name in ("exp_avg_scale", "exp_avg_sq_scale")}
+        if self._settings["master"] and any(p.dtype != torch.float32 for p in params):
+            scales["master"] = [st.get("master") if p.dtype != torch.float32 else None for p, st in zip(params, states)]
+        plan = K.AdamWPlan([p.data for p in params], [st["exp_avg"] for st in states], [st["exp_avg_sq"] for st in states], **scales)
+        device = params[0].device if self._counts_on_device(group) else torch.device("cpu")
+        by_value = {}
+        for k, st in enumerate(states):
+            by_value.setdefault(float(st.get("step", 0.0)), []).append(k)
+        cohorts = []
+        for value, members in by_value.items():
+            c = _Cohort(torch.tensor(value, dtype=torch.float32, device=device), members)
+            for k in members:
+                states[k]["step"] = c.step
+            cohorts.append(c)
+        return _Group(params, plan, states, cohorts)
+
+    def _group(self, index, group):
+        g = self._plans.get(index)
+        if g is not None and len(g.params) == len(group["params"]):
+            state = self.state
+            for p, q, at, n, (st, m, v, step) in zip(group["params"], g.params, g.at, g.plan.numels, g.kept):
+                if p is not q or p.data_ptr() != at or p.numel() != n or state.get(p) is not st or st["exp_avg"] is not m or st["exp_avg_sq"] is not v or st["step"] is not step:
+                    break
+            else:
+                return g
+        g = self._plans[index] = self._make(group)
+        return g
+
+    # -- the update ----------------------------------------------------------------------------------------------------------
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        work, norms = [], []
+        for index, group in enumerate(self.param_groups):
+            if group.get("amsgrad") or group.get("maximize") or group.get("differentiable"):
+                raise NotImplementedError("FusedAdamW: amsgrad, maximize and differentiable are not built")
+            if not group["params"]:
+                continue
+            g = self._group(index, group)
+            grads = [self._gradient(p, n) for p, n in zip(g.params, g.plan.numels)]
+            if all(x is None for x in grads):
+                continue
+            if any(x is None for x in grads):
+                self._split(g, grads)
+            whole = K.GradList.of_checked(grads, g.plan)
+            norms.append(whole)
+            for c in g.cohorts:
+                if grads[c.members[0]] is None:
+                    continue
+                if len(c.members) == len(grads):
+                    part = whole
+                else:
+                    mine = set(c.members)
+                    part = K.GradList.of_checked([x if k in mine else None for k, x in enumerate(grads)], g.plan)
+                work.append((index, group, g, c, part))
+        if not work:
+            return loss
+        guard = self._settings["guard_range"]
+        words = None
+        on_device = [c.step for _, group, _, c, _ in work if self._counts_on_device(group)]
+        if self.max_norm is not None:
+            if self.grad_norm is None:
+                self.grad_norm = torch.zeros(4, dtype=torch.float32, device=norms[0].device)
+            words = K.grad_norm(norms, self.max_norm, out=self.grad_norm, counters=on_device[:64], guard_range=guard)
+            on_device = on_device[64:]
+        for s in on_device:
+            K.adamw_count(s, norm=words, guard_range=guard)
+        for index, group, g, c, part in work:
+            host = not self._counts_on_device(group)
+            t = int(c.step.item()) + 1 if host else c.step
+            K.adamw_step(g.plan, part, group["lr"], t, group["betas"], group["eps"], group["weight_decay"], norm=words,
+                         seed=self._settings["seed"] + index * 0x9E3779B97F4A7C15, guard_range=guard)
+            if host:
+                c.step += 1.0
+        return loss
+
+    @staticmethod
+    def _gradient(p, n):
+        x = p.grad
+        if x is None:
+            return None
+        if x.layout is not torch.strided:
+            raise NotImplementedError("FusedAdamW: sparse gradients")
+        if x.numel() != n or x.get_device() != p.get_device():      # p.data was replaced by something else behind its gradient
+            raise RuntimeError("FusedAdamW: a gradient has another size or device than its parameter")
+        return x if x.is_contiguous() else x.contiguous()
+
+    def _split(self, g, grads):
+        """Cohorts in which only some have a gradient this time part: the others' counter stays."""
+        for c in list(g.cohorts):
+            have = [k for k in c.members if grads[k] is not None]
+            if have and len(have) < len(c.members):
+                c.members = [k for k in c.members if grads[k] is None]
+                new = _Cohort(c.step.clone(), have)
+                for k in have:
+                    g.states[k]["step"] = new.step
+                    g.kept[k] = g.kept[k][:3] + (new.step,)
+                g.cohorts.append(new)

@@ -39,10 +39,10 @@ extern "C" {
 typedef void* benerf_stream_t; /* hipStream_t */
 
 /* ABI revision of this header: bumped whenever the signature or the argument meaning of an entry point changes (round 5's
- * `params` argument in front of benerf_mlp_bwd_dw made it 101; round 6: 102, 103 with the loss-glue operators).  benerf_version() returns the revision the LIBRARY
+ * `params` argument in front of benerf_mlp_bwd_dw made it 101; round 6: 102, 103 with the loss-glue operators; 104: the optimiser over lists of tensors).  benerf_version() returns the revision the LIBRARY
  * was built from - a binding compares the two before its first call (benerf_amd/_lib.py does and refuses a mismatch): a caller
  * compiled against another revision would pass shifted arguments. */
-#define BENERF_ABI_VERSION 103
+#define BENERF_ABI_VERSION 104
 int benerf_version(void);
 const char* benerf_last_error(void);
 
@@ -399,6 +399,63 @@ int benerf_gather_rows(const float* src, const int64_t* idx, int64_t n_idx, int 
 int benerf_adam_step(float* param, const float* grad, float* exp_avg, float* exp_avg_sq,
                      int64_t n, double lr, double beta1, double beta2, double eps, int step,
                      double grad_scale, const uint32_t* skip_if_range, benerf_stream_t stream);
+
+/* ---------------------------------------------------------------- K9: optimiser over lists of tensors */
+/* AdamW (decoupled decay) over many tensors at once, where they live, with moments in 32 or in 8 bits, and the gradient norm of the
+ * same list with a clip coefficient and a verdict that AdamW takes on the device.  Formulas: csrc/adamw.hip.
+ *
+ * A PLAN describes the list: benerf_adamw_plan_fill writes it into host memory of benerf_adamw_plan_bytes(...) bytes, the caller
+ * copies these bytes to the device once and hands both copies to every call.  Gradients are not part of it: every call takes a HOST
+ * array of n_tensors device pointers (NULL: no gradient this time, the tensor and its moments are left alone), which travel in the
+ * launch - a captured launch keeps the addresses it was captured with.  The tensors of a plan must not overlap.
+ *   state_bits 32: exp_avg, exp_avg_sq float32 [n], the scale pointers are not read;
+ *   state_bits 8:  exp_avg uint8 [n] e4m3 codes of m, exp_avg_sq uint8 [n] e4m3 codes of sqrt(v), *_scale float32 [ceil(n / 128)]: the
+ *                  power of two that belongs to 128 consecutive elements (0 moments: any scale with codes 0);
+ *   state_bits 0:  a plan for benerf_grad_norm_partial alone, only n is read.
+ *   master: float32 [n], or NULL: the parameter itself is read.  With it, param is written only.
+ *   first_block: number of the tensor's first block of 128 in the caller's numbering (8 bits: the generator's counter; give every
+ *                tensor its own range).
+ * Element types of parameters and gradients: BENERF_F32 / _BF16 / _F16, one of each per plan / call.  Pointers need the alignment of
+ * an element.  n = 0 is allowed. */
+enum { BENERF_F32 = 0, BENERF_BF16 = 1, BENERF_F16 = 2 };
+enum { BENERF_ADAMW_BLOCK = 128 };
+typedef struct BenerfAdamwTensor {
+    void* param;
+    void* exp_avg;
+    void* exp_avg_sq;
+    float* exp_avg_scale;
+    float* exp_avg_sq_scale;
+    float* master;
+    int64_t n;
+    int64_t first_block;
+} BenerfAdamwTensor;
+typedef struct BenerfAdamwCfg {
+    double lr, beta1, beta2, eps, weight_decay;
+    double grad_scale;       /* multiplies every gradient first */
+    int64_t step;            /* t of this step, from 1; not read with step_dev */
+    uint64_t seed;           /* stochastic rounding of 8-bit moments */
+    const float* lr_dev;     /* NULL, or one device float that takes the place of lr */
+    const float* step_dev;   /* NULL, or one device float that holds t of this step (benerf_adamw_count / benerf_grad_norm_finish count) */
+} BenerfAdamwCfg;
+size_t benerf_adamw_plan_bytes(const BenerfAdamwTensor* tensors_host, int n_tensors);       /* 0: bad list */
+int benerf_adamw_plan_fill(const BenerfAdamwTensor* tensors_host, int n_tensors, int param_type, int state_bits, void* plan_host,
+                           size_t plan_bytes);
+/* One step over the list.  norm_words: NULL, or what benerf_grad_norm_finish wrote: gradients are multiplied by [1], nothing happens
+ * where [2] is set, and without step_dev t = step - [3].  skip_if_range: as in benerf_adam_step (status words, or NULL). */
+int benerf_adamw_step(const void* plan_host, const void* plan_dev, const void* const* grads_host, int grad_type,
+                      const BenerfAdamwCfg* cfg, const float* norm_words, const uint32_t* skip_if_range, benerf_stream_t stream);
+/* *step_dev += 1, unless norm_words or skip_if_range say that the step is skipped: for captured steps without a norm. */
+int benerf_adamw_count(float* step_dev, const float* norm_words, const uint32_t* skip_if_range, benerf_stream_t stream);
+/* Squares of the list's gradients, summed in f64 and in a fixed order, one partial sum per workgroup into partials (device, room for
+ * benerf_grad_norm_partials(plan)); *used_host: how many were written.  Several lists (types, groups) write one behind the other. */
+size_t benerf_grad_norm_partials(const void* plan_host);
+int benerf_grad_norm_partial(const void* plan_host, const void* plan_dev, const void* const* grads_host, int grad_type,
+                             double* partials, size_t n_partials, int64_t* used_host, benerf_stream_t stream);
+/* words[4] = { norm = |grad_scale| sqrt(sum), coefficient min(1, max_norm / (norm + 1e-6)), 1 if the step is to be skipped (norm inf or
+ * NaN, or the status words say so) else 0, number of skipped steps (accumulate: added to what words[3] holds) }.  max_norm > 0, may be
+ * infinite.  counters_host: up to 64 step counters (device floats) that go up by one unless the step is skipped. */
+int benerf_grad_norm_finish(const double* partials, int64_t n_partials, double max_norm, double grad_scale, float* words, int accumulate,
+                            const uint32_t* skip_if_range, float* const* counters_host, int n_counters, benerf_stream_t stream);
 
 #ifdef __cplusplus
 }
