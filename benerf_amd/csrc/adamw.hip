@@ -16,39 +16,52 @@
 #include "common.h"
 #include <math.h>
 #include <string.h>
+#include <type_traits>
 
 namespace {
 
-constexpr int THREADS = 256;
+constexpr int THREADS = 128;
 constexpr int BLOCK = BENERF_ADAMW_BLOCK;
+constexpr int CHUNK = THREADS * 4;           // elements a workgroup of the step takes: four a thread
+constexpr int64_t PAST_BYTES = 256ll << 20;  // what the memory-side cache holds
 constexpr uint32_t PLAN_MAGIC = 0x41445731u;
 static_assert(BLOCK == 128, "a block is half a wavefront of four elements a lane");
 
-// The plan: what a launch needs to find its way through the list, filled on the host, uploaded once.
-struct Entry {
-    void* param;
+// The plan: what a launch needs to find its way through the list, filled on the host, uploaded once.  A workgroup takes a chunk and reads
+// everything about it in one record - its data's addresses are one load away, not three.
+struct Entry {                // one per tensor, for the host
+    int64_t n;
+    int64_t first_chunk;
+};
+struct Chunk {
+    void* param;              // of the chunk's first element
     void* m;
     void* v;
     float* ms;
     float* vs;
     float* master;
-    int64_t n;
-    int64_t first_block;      // number of the tensor's first block of 128 in the list: the generator's counter
-    int64_t first_chunk;
+    int64_t block;            // number of its first block of 128 in the list: the generator's counter
+    int32_t tensor;
+    int32_t index;            // of the chunk in its tensor
+    int32_t count;            // elements
+    int32_t pad[3];
 };
+static_assert(sizeof(Chunk) == 80, "a multiple of 16 bytes");
 struct PlanHead {
     uint32_t magic;
     int32_t n_tensors;
     int32_t param_type, state_bits, has_master;
-    int32_t unroll;           // a chunk is THREADS * 4 * unroll elements: one workgroup
+    int32_t shape;            // SHORT ..: how it is launched and read
+    int32_t pad;
     int64_t n_chunks;
-    int64_t map_at;           // byte offset of int32 map[n_chunks]: the tensor of every chunk
+    int64_t chunks_at;        // byte offset of the chunks' records
     int64_t bytes;
 };
 constexpr size_t HEAD_BYTES = 64;
 static_assert(sizeof(PlanHead) <= HEAD_BYTES, "plan header");
 
-__host__ __device__ inline const Entry* plan_entries(const void* plan) { return reinterpret_cast<const Entry*>(static_cast<const char*>(plan) + HEAD_BYTES); }
+inline const Entry* plan_entries(const void* plan) { return reinterpret_cast<const Entry*>(static_cast<const char*>(plan) + HEAD_BYTES); }
+inline const Chunk* plan_chunks_dev(const void* plan_dev, const PlanHead* h) { return reinterpret_cast<const Chunk*>(static_cast<const char*>(plan_dev) + h->chunks_at); }
 
 // Gradients change from step to step while the rest of the list stays: their addresses travel in the launch itself, so that a captured
 // launch keeps its own and nothing on the device has to be rewritten.  4 KiB is what a launch may carry.
@@ -62,11 +75,8 @@ struct Hyper {
     float gs, decay, step_size, omb1, b2, omb2, eps, inv_bc2;
 };
 struct AdamwArgs {
-    const Entry* entries;
-    const int32_t* map;
-    int64_t chunk0;            // first chunk of this launch
-    int32_t tensor0;           // first tensor of this launch
-    int32_t unroll;
+    const Chunk* chunks;       // of this launch
+    int64_t tensor0;           // first tensor of this launch
     Hyper h;                   // for t = step, lr from the host
     const float* norm;         // [4] of the norm operator, or null
     const uint32_t* status;    // range guard words, or null
@@ -113,208 +123,260 @@ __device__ __forceinline__ bool step_scalars(const AdamwArgs& a, Hyper& h, int64
 }
 
 // ---- four consecutive elements, at any element-aligned address -------------------------------------------------------------
-typedef float float4u __attribute__((ext_vector_type(4), aligned(4)));
-typedef unsigned short ushort4v __attribute__((ext_vector_type(4)));
-typedef unsigned short ushort4u __attribute__((ext_vector_type(4), aligned(2)));
 typedef _Float16 half4v __attribute__((ext_vector_type(4)));
 typedef __bf16 bf4v __attribute__((ext_vector_type(4)));
 typedef float float4v __attribute__((ext_vector_type(4)));
 typedef uint32_t u32u __attribute__((aligned(1)));
+// addresses come out of the plan: say that they are global memory's, or every access becomes a flat one
+// PAST: past the caches, for lists that no cache holds until the next step
+template <typename T, bool PAST = false>
+__device__ __forceinline__ T get(const void* p, int64_t i) {
+    typedef const __attribute__((address_space(1))) T* at;
+    const T* q = static_cast<const T*>(p) + i;
+    if constexpr (PAST) return __builtin_nontemporal_load((at)q);
+    else return *(at)q;
+}
+template <typename T, bool PAST = false>
+__device__ __forceinline__ void put(void* p, int64_t i, T x) {
+    typedef __attribute__((address_space(1))) T* at;
+    T* q = static_cast<T*>(p) + i;
+    if constexpr (PAST) __builtin_nontemporal_store(x, (at)q);
+    else *(at)q = x;
+}
 
-struct F32 {
-    typedef float4v raw;
-    static constexpr bool NARROW = false;
-    __device__ static raw load(const void* p, int64_t i) { return *reinterpret_cast<const float4u*>(static_cast<const float*>(p) + i); }
-    __device__ static raw load_part(const void* p, int64_t i, int k) {
-        raw r = 0.f;
-        for (int j = 0; j < 4; ++j)
-            if (j < k) r[j] = static_cast<const float*>(p)[i + j];
-        return r;
-    }
-    __device__ static float4v widen(raw r) { return r; }
-    __device__ static raw narrow(float4v x) { return x; }
-    __device__ static void store(void* p, int64_t i, raw r) { *reinterpret_cast<float4u*>(static_cast<float*>(p) + i) = r; }
-    __device__ static void store_part(void* p, int64_t i, int k, raw r) {
-        for (int j = 0; j < 4; ++j)
-            if (j < k) static_cast<float*>(p)[i + j] = r[j];
-    }
-};
-template <typename V>
-struct Half16 {       // bf16 and f16: rounded to nearest even, once
-    typedef ushort4v raw;
-    static constexpr bool NARROW = true;
-    __device__ static raw load(const void* p, int64_t i) { return *reinterpret_cast<const ushort4u*>(static_cast<const unsigned short*>(p) + i); }
-    __device__ static raw load_part(const void* p, int64_t i, int k) {
+// V: a vector of four; raw: its bits in memory.  k of the four elements from i on are there.
+template <typename E, typename V>
+struct Four {
+    typedef E raw __attribute__((ext_vector_type(4)));
+    typedef E unaligned __attribute__((ext_vector_type(4), aligned(sizeof(E))));
+    static constexpr bool NARROW = sizeof(E) < 4;       // rounded to nearest even, once, when stored
+    static constexpr int BYTES = sizeof(E);
+    template <bool PAST>
+    __device__ static raw load(const void* p, int i, int k) {
+        if (k >= 4) return get<unaligned, PAST>(static_cast<const E*>(p) + i, 0);
         raw r = 0;
-        for (int j = 0; j < 4; ++j)
-            if (j < k) r[j] = static_cast<const unsigned short*>(p)[i + j];
+        for (int j = 0; j < 3; ++j)
+            if (j < k) r[j] = get<E>(p, i + j);
         return r;
+    }
+    template <bool PAST>
+    __device__ static void store(void* p, int i, int k, raw r) {
+        if (k >= 4) return put<unaligned, PAST>(static_cast<E*>(p) + i, 0, r);
+        for (int j = 0; j < 3; ++j)
+            if (j < k) put<E>(p, i + j, r[j]);
     }
     __device__ static float4v widen(raw r) { return __builtin_convertvector(__builtin_bit_cast(V, r), float4v); }
     __device__ static raw narrow(float4v x) { return __builtin_bit_cast(raw, __builtin_convertvector(x, V)); }
-    __device__ static void store(void* p, int64_t i, raw r) { *reinterpret_cast<ushort4u*>(static_cast<unsigned short*>(p) + i) = r; }
-    __device__ static void store_part(void* p, int64_t i, int k, raw r) {
-        for (int j = 0; j < 4; ++j)
-            if (j < k) static_cast<unsigned short*>(p)[i + j] = r[j];
+};
+typedef Four<float, float4v> F32;
+typedef Four<unsigned short, bf4v> BF16;
+typedef Four<unsigned short, half4v> F16;
+
+// ---- moments in 32 bits --------------------------------------------------------------------------------------------------------
+// Four elements from i on, k of them there; loads and arithmetic apart, so that a chunk's loads can all be on their way first.
+template <class PT, class GT, bool MASTER, bool PAST>
+struct Four32 {
+    typename PT::raw p;
+    typename GT::raw g;
+    float4v w, m, v;
+
+    __device__ __forceinline__ void load(const Chunk& c, const void* gp, int i, int k) {
+        if (MASTER) w = F32::load<PAST>(c.master, i, k);
+        else p = PT::template load<PAST>(c.param, i, k);
+        g = GT::template load<PAST>(gp, i, k);
+        m = F32::load<PAST>(c.m, i, k);
+        v = F32::load<PAST>(c.v, i, k);
+    }
+    // root and quotient correctly rounded: 60 instructions an element more than their approximations would take, of 200 that the memory
+    // leaves time for
+    __device__ __forceinline__ void update(const Hyper& h) {
+        if (!MASTER) w = PT::widen(p);
+        const float4v x = GT::widen(g);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float gj = x[j] * h.gs;
+            m[j] = m[j] + (gj - m[j]) * h.omb1;
+            v[j] = v[j] * h.b2 + (gj * gj) * h.omb2;
+            w[j] = w[j] * h.decay - h.step_size * (m[j] / (sqrtf(v[j]) * h.inv_bc2 + h.eps));
+        }
+    }
+    __device__ __forceinline__ void store(const Chunk& c, int i, int k) const {
+        if (MASTER) F32::store<PAST>(c.master, i, k, w);
+        PT::template store<PAST>(c.param, i, k, PT::narrow(w));
+        F32::store<PAST>(c.m, i, k, m);
+        F32::store<PAST>(c.v, i, k, v);
     }
 };
-typedef Half16<bf4v> BF16;
-typedef Half16<half4v> F16;
 
-// the update of four elements; v: v itself (32 bits) or, rooted, computed from u by the caller.  Returns the root of the new v.
-__device__ __forceinline__ void update(float4v& p, float4v g, float4v& m, float4v& v, float4v& root, const Hyper& h) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const float x = g[j] * h.gs;
-        m[j] = m[j] + (x - m[j]) * h.omb1;
-        v[j] = v[j] * h.b2 + (x * x) * h.omb2;
-        root[j] = sqrtf(v[j]);
-        p[j] = p[j] * h.decay - h.step_size * (m[j] / (root[j] * h.inv_bc2 + h.eps));
-    }
-}
-
-template <class PT, class GT, bool MASTER>
-__device__ __forceinline__ void four32(const Entry& e, const void* gp, int64_t i, int k, const Hyper& h) {
-    const bool full = k >= 4;
-    float4v p = MASTER ? (full ? F32::load(e.master, i) : F32::load_part(e.master, i, k))
-                       : PT::widen(full ? PT::load(e.param, i) : PT::load_part(e.param, i, k));
-    const float4v g = GT::widen(full ? GT::load(gp, i) : GT::load_part(gp, i, k));
-    float4v m = full ? F32::load(e.m, i) : F32::load_part(e.m, i, k);
-    float4v v = full ? F32::load(e.v, i) : F32::load_part(e.v, i, k);
-    float4v root;
-    update(p, g, m, v, root, h);
-    if (full) {
-        if (MASTER) F32::store(e.master, i, p);
-        PT::store(e.param, i, PT::narrow(p));
-        F32::store(e.m, i, m);
-        F32::store(e.v, i, v);
-    } else {
-        if (MASTER) F32::store_part(e.master, i, k, p);
-        PT::store_part(e.param, i, k, PT::narrow(p));
-        F32::store_part(e.m, i, k, m);
-        F32::store_part(e.v, i, k, v);
-    }
-}
-
-// ---- 8-bit moments ---------------------------------------------------------------------------------------------------------
+// ---- moments in 8 bits -----------------------------------------------------------------------------------------------------------
 __device__ __forceinline__ float4v decode4(uint32_t w, float s) {
     const auto a = __builtin_amdgcn_cvt_pk_f32_fp8(w, false), b = __builtin_amdgcn_cvt_pk_f32_fp8(w, true);
     return float4v{a[0] * s, a[1] * s, b[0] * s, b[1] * s};
-}
-// high 16 bits of |x|, 0 for inf and NaN: they must not take the block's other values along
-__device__ __forceinline__ uint32_t top16(float x) {
-    const uint32_t b = __float_as_uint(x) & 0x7fffffffu;
-    return b < 0x7f800000u ? b : 0u;
 }
 __device__ __forceinline__ uint32_t pk_max(uint32_t a, uint32_t b) {
     typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
     return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, a), __builtin_bit_cast(u16x2, b)));
 }
-// maximum of both 16-bit halves over the 32 lanes of a block
+// maximum of both 16-bit halves over the 32 lanes of a block: four steps inside a row of 16, one between two rows
 __device__ __forceinline__ uint32_t block_max(uint32_t x) {
-    for (int d = 1; d < 32; d <<= 1) x = pk_max(x, (uint32_t)__shfl_xor((int)x, d, 32));
-    return x;
+    x = pk_max(x, (uint32_t)__builtin_amdgcn_mov_dpp((int)x, 0xB1, 0xf, 0xf, true));       // lane ^ 1
+    x = pk_max(x, (uint32_t)__builtin_amdgcn_mov_dpp((int)x, 0x4E, 0xf, 0xf, true));       // lane ^ 2
+    x = pk_max(x, (uint32_t)__builtin_amdgcn_mov_dpp((int)x, 0x124, 0xf, 0xf, true));      // a quad on
+    x = pk_max(x, (uint32_t)__builtin_amdgcn_mov_dpp((int)x, 0x128, 0xf, 0xf, true));      // half a row on
+    const auto r = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+    return pk_max(r[0], r[1]);
 }
-// x scaled by inv, rounded to the e4m3 grid with the draw h16; keep: a value that is not 0 stays so
-__device__ __forceinline__ float to_grid(float x, float inv, uint32_t h16, bool keep) {
-    const float y = fabsf(x) * inv;
-    const uint32_t b = __float_as_uint(y);
-    if (!(b < 0x7f800000u)) return __uint_as_float(0x7fc00000u);
-    float q;
-    if (b >= 0x3c800000u) {               // from 2^-6 on: three bits behind the leading one
-        q = __uint_as_float((b + (h16 << 4)) & 0xfff00000u);
-    } else {                              // below: steps of 2^-9
-        float k = floorf(y * 512.f + (float)h16 * (1.f / 65536.f));
-        if (keep && y > 0.f) k = fmaxf(k, 1.f);
-        q = k * (1.f / 512.f);
-    }
-    return copysignf(q, x);
+// |x| / scale on the e4m3 grid (steps of 2^(E - 3), 2^-9 from below 2^-6 on), down after the draw h / 2^16 is added: the draw goes into the
+// 20 bits behind the grid's three, which are then cut off - a carry is the step up.  Below 2^-6 the same happens 2^-6 higher up, where the
+// grid has the right step.  The scale is a power of two, so nothing else is rounded (but what 2^-6 + y loses: 2^-21 of a step).  inf and the
+// NaN of 0x7fc00000 come out as such, the conversion makes both NaN.
+__device__ __forceinline__ float to_grid(float x, float low, float inv, uint32_t h) {
+    const float c = x < low ? 1.f / 64.f : 0.f;
+    const uint32_t z = __float_as_uint(__builtin_fmaf(x, inv, c)) + (h << 4);
+    return __uint_as_float(z & 0xfff00000u) - c;
 }
-__device__ __forceinline__ uint32_t encode4(float4v x, float inv, const uint32_t (&h16)[4], bool keep) {
-    int w = 0;
-    w = __builtin_amdgcn_cvt_pk_fp8_f32(to_grid(x[0], inv, h16[0], keep), to_grid(x[1], inv, h16[1], keep), w, false);
-    w = __builtin_amdgcn_cvt_pk_fp8_f32(to_grid(x[2], inv, h16[2], keep), to_grid(x[3], inv, h16[3], keep), w, true);
-    return (uint32_t)w;
-}
-__device__ __forceinline__ uint32_t load_codes(const void* p, int64_t i, int k) {
-    if (k >= 4) return *reinterpret_cast<const u32u*>(static_cast<const uint8_t*>(p) + i);
+template <bool PAST>
+__device__ __forceinline__ uint32_t load_codes(const void* p, int i, int k) {
+    if (k >= 4) return get<u32u, PAST>(static_cast<const uint8_t*>(p) + i, 0);
     uint32_t w = 0;
     for (int j = 0; j < 3; ++j)
-        if (j < k) w |= (uint32_t) static_cast<const uint8_t*>(p)[i + j] << (8 * j);
+        if (j < k) w |= (uint32_t)get<uint8_t>(p, i + j) << (8 * j);
     return w;
 }
-__device__ __forceinline__ void store_codes(void* p, int64_t i, int k, uint32_t w) {
+template <bool PAST>
+__device__ __forceinline__ void store_codes(void* p, int i, int k, uint32_t w) {
     if (k >= 4) {
-        *reinterpret_cast<u32u*>(static_cast<uint8_t*>(p) + i) = w;
+        put<u32u, PAST>(static_cast<uint8_t*>(p) + i, 0, w);
         return;
     }
     for (int j = 0; j < 3; ++j)
-        if (j < k) static_cast<uint8_t*>(p)[i + j] = (uint8_t)(w >> (8 * j));
+        if (j < k) put<uint8_t>(p, i + j, (uint8_t)(w >> (8 * j)));
 }
-
-// Called by whole wavefronts: a lane behind the tensor's end (k <= 0) takes part in the block's maximum with zeros.
-template <class PT, class GT, bool MASTER>
-__device__ __forceinline__ void four8(const Entry& e, const void* gp, int64_t i, int k, const Hyper& h, int64_t t, uint64_t seed) {
-    const bool live = k > 0, full = k >= 4;
-    float4v p = 0.f, g = 0.f, m = 0.f, v = 0.f, root = 0.f;
-    const int64_t blk = i >> 7;
-    if (live) {
-        p = MASTER ? (full ? F32::load(e.master, i) : F32::load_part(e.master, i, k)) : PT::widen(full ? PT::load(e.param, i) : PT::load_part(e.param, i, k));
-        g = GT::widen(full ? GT::load(gp, i) : GT::load_part(gp, i, k));
-        m = decode4(load_codes(e.m, i, k), e.ms[blk]);
-        const float4v u = decode4(load_codes(e.v, i, k), e.vs[blk]);
-        v = u * u;
-        update(p, g, m, v, root, h);
-    }
-    uint32_t mx = 0, ux = 0;
+__device__ __forceinline__ uint32_t pack_tops(uint32_t m, uint32_t u) { return __builtin_amdgcn_perm(m, u, 0x07060302u); }
+// bits of |x|: the highest of four, and where only finite ones count
+__device__ __forceinline__ uint32_t top_bits(float4v x) {
+    return max(max(__float_as_uint(x[0]), __float_as_uint(x[1])), max(__float_as_uint(x[2]), __float_as_uint(x[3])));
+}
+__device__ __forceinline__ uint32_t finite_top(float4v x) {
+    uint32_t top = 0;
+    for (int j = 0; j < 4; ++j) top = fabsf(x[j]) < INFINITY ? max(top, __float_as_uint(fabsf(x[j]))) : top;
+    return top;
+}
+// Philox4x32-10 as in common.h, its products as 32 x 32 -> 64 bits and its sums of three as one instruction each: the step is bound by
+// vector instructions, and this is the longest part of them
+__device__ __forceinline__ uint4 draws4(int64_t group, uint32_t t, uint2 key) {
+    uint32_t x = (uint32_t)group, y = (uint32_t)(group >> 32), z = t, w = 0x40000000u;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        mx = max(mx, top16(m[j]));
-        ux = max(ux, top16(root[j]));
+    for (int r = 0; r < 10; ++r) {
+        const uint64_t a = (uint64_t)x * 0xD2511F53u, b = (uint64_t)z * 0xCD9E8D57u;
+        x = __builtin_amdgcn_bitop3_b32((uint32_t)(b >> 32), y, key.x, 0x96);
+        z = __builtin_amdgcn_bitop3_b32((uint32_t)(a >> 32), w, key.y, 0x96);
+        y = (uint32_t)b;
+        w = (uint32_t)a;
+        key.x += 0x9E3779B9u;
+        key.y += 0xBB67AE85u;
     }
-    const uint32_t top = block_max((mx & 0xffff0000u) | (ux >> 16));
-    if (!live) return;
-    const uint32_t em = max(top >> 23, 27u), eu = max((top & 0xffffu) >> 7, 27u);
-    const int64_t c = (e.first_block * BLOCK + i) >> 2;
-    const uint4 r = philox4x32_10(make_uint4((uint32_t)c, (uint32_t)(c >> 32), (uint32_t)t, 0x40000000u), make_uint2((uint32_t)seed, (uint32_t)(seed >> 32)));
-    const uint32_t lo[4] = {r.x & 0xffffu, r.y & 0xffffu, r.z & 0xffffu, r.w & 0xffffu}, hi[4] = {r.x >> 16, r.y >> 16, r.z >> 16, r.w >> 16};
-    store_codes(e.m, i, k, encode4(m, __uint_as_float((261u - em) << 23), lo, false));
-    store_codes(e.v, i, k, encode4(root, __uint_as_float((261u - eu) << 23), hi, true));
-    if ((i & (BLOCK - 1)) == 0) {
-        e.ms[blk] = __uint_as_float((em - 7u) << 23);
-        e.vs[blk] = __uint_as_float((eu - 7u) << 23);
-    }
-    if (full) {
-        if (MASTER) F32::store(e.master, i, p);
-        PT::store(e.param, i, PT::narrow(p));
-    } else {
-        if (MASTER) F32::store_part(e.master, i, k, p);
-        PT::store_part(e.param, i, k, PT::narrow(p));
-    }
+    return make_uint4(x, y, z, w);
 }
 
-// One workgroup per chunk.
-template <class PT, class GT, int BITS, bool MASTER, int N>
+// Called by whole wavefronts: a lane behind the end takes part in its block's maximum with zeros.
+template <class PT, class GT, bool MASTER, bool PAST>
+struct Four8 {
+    typename PT::raw p;
+    typename GT::raw g;
+    float4v w;
+    uint32_t mw, uw;          // codes, before and after the update
+    float ms, us;             // scales, likewise
+
+    __device__ __forceinline__ void load(const Chunk& c, const void* gp, int i, int k) {
+        if (MASTER) w = F32::load<PAST>(c.master, i, k);
+        else p = PT::template load<PAST>(c.param, i, k);
+        g = GT::template load<PAST>(gp, i, k);
+        mw = load_codes<PAST>(c.m, i, k);
+        uw = load_codes<PAST>(c.v, i, k);
+        ms = k > 0 ? get<float>(c.ms, i >> 7) : 0.f;
+        us = k > 0 ? get<float>(c.vs, i >> 7) : 0.f;
+    }
+    __device__ __forceinline__ void update(const Hyper& h, int64_t group, uint32_t t, uint2 key) {
+        if (!MASTER) w = PT::widen(p);
+        const float4v x = GT::widen(g);
+        float4v m = decode4(mw, ms), v, root;
+        const float4v u = decode4(uw, us);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float gj = x[j] * h.gs;
+            m[j] = m[j] + (gj - m[j]) * h.omb1;
+            v[j] = (u[j] * u[j]) * h.b2 + (gj * gj) * h.omb2;
+            root[j] = __builtin_amdgcn_sqrtf(v[j]);              // to 1 ulp: the code has 4 bits
+        }
+        uint32_t top = block_max(pack_tops(__float_as_uint(fmaxf(fmaxf(fabsf(m[0]), fabsf(m[1])), fmaxf(fabsf(m[2]), fabsf(m[3])))), top_bits(root)));
+        // The instruction takes denormal numbers for 0: their roots (below 2^-63) count where nothing else in the block does, or with an eps
+        // that they are not lost in.
+        if (h.eps < 1e-11f || __any((top & 0xffffu) == 0u)) {
+            for (int j = 0; j < 4; ++j) root[j] = sqrtf(v[j]);
+            top = block_max(pack_tops(finite_top(m), finite_top(root)));
+        }
+        // inf or NaN (NaN in m comes with one in v): it must not take the block's other values along
+        if (__any((top & 0x7f80u) == 0x7f80u || (top & 0x7f800000u) == 0x7f800000u)) {
+            top = block_max(pack_tops(finite_top(m), finite_top(root)));
+            for (int j = 0; j < 4; ++j) {
+                m[j] = m[j] == m[j] ? m[j] : __uint_as_float(0x7fc00000u);
+                root[j] = root[j] == root[j] ? root[j] : __uint_as_float(0x7fc00000u);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            w[j] = __builtin_fmaf(-h.step_size, m[j] * __builtin_amdgcn_rcpf(__builtin_fmaf(root[j], h.inv_bc2, h.eps)), w[j] * h.decay);
+        const uint32_t em = max(top >> 23, 27u), eu = max(top >> 7 & 0xffu, 27u);
+        ms = __uint_as_float((em - 7u) << 23);
+        us = __uint_as_float((eu - 7u) << 23);
+        const float im = __uint_as_float((261u - em) << 23), iu = __uint_as_float((261u - eu) << 23);
+        const float lm = __uint_as_float((em - 13u) << 23), lu = __uint_as_float((eu - 13u) << 23), least = __uint_as_float((eu - 16u) << 23);
+        const uint4 r = draws4(group, t, key);
+        const uint32_t rw[4] = {r.x, r.y, r.z, r.w};
+        float a[4], b[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            a[j] = copysignf(to_grid(fabsf(m[j]), lm, im, rw[j] & 0xffffu), m[j]);
+            // one step is the least that a value above 0 may become: lifted to it, it stays there whatever the draw
+            const float lifted = root[j] < least ? (v[j] > 0.f ? least : 0.f) : root[j];
+            b[j] = to_grid(lifted, lu, iu, rw[j] >> 16);
+        }
+        mw = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(a[2], a[3], __builtin_amdgcn_cvt_pk_fp8_f32(a[0], a[1], 0, false), true);
+        uw = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(b[2], b[3], __builtin_amdgcn_cvt_pk_fp8_f32(b[0], b[1], 0, false), true);
+    }
+    __device__ __forceinline__ void store(const Chunk& c, int i, int k) const {
+        if (MASTER) F32::store<PAST>(c.master, i, k, w);
+        PT::template store<PAST>(c.param, i, k, PT::narrow(w));
+        store_codes<PAST>(c.m, i, k, mw);
+        store_codes<PAST>(c.v, i, k, uw);
+        if (k > 0 && (i & (BLOCK - 1)) == 0) {
+            put<float>(c.ms, i >> 7, ms);
+            put<float>(c.vs, i >> 7, us);
+        }
+    }
+};
+
+// One workgroup per chunk, four elements a thread.
+template <class PT, class GT, int BITS, bool MASTER, int N, bool PAST>
 __global__ __launch_bounds__(THREADS) void adamw_kernel(AdamwArgs a, Ptrs<N> grads) {
-    const int64_t chunk = a.chunk0 + blockIdx.x;
-    const int tensor = a.map[chunk];
-    const void* gp = grads.p[tensor - a.tensor0];
+    const Chunk c = a.chunks[blockIdx.x];
+    const char* gp = static_cast<const char*>(grads.p[c.tensor - a.tensor0]);
     if (!gp) return;
+    gp += (int64_t)c.index * CHUNK * GT::BYTES;
     Hyper h;
     int64_t t;
     if (!step_scalars(a, h, t)) return;
-    const Entry e = a.entries[tensor];
-    const int64_t base = (chunk - e.first_chunk) * ((int64_t)THREADS * 4 * a.unroll);
-    for (int s = 0; s < a.unroll; ++s) {
-        const int64_t i = base + (int64_t)(s * THREADS + threadIdx.x) * 4;
-        const int64_t left = e.n - i;
-        const int k = left >= 4 ? 4 : (int)left;
-        if (BITS == 8) {
-            four8<PT, GT, MASTER>(e, gp, i, k, h, t, a.seed);
-        } else if (k > 0) {
-            four32<PT, GT, MASTER>(e, gp, i, k, h);
-        }
-    }
+    const int i = threadIdx.x * 4;
+    typename std::conditional<BITS == 8, Four8<PT, GT, MASTER, PAST>, Four32<PT, GT, MASTER, PAST>>::type f;
+    auto chunk = [&](int here) {              // elements there from i on
+        f.load(c, gp, i, here);
+        if constexpr (BITS == 8) f.update(h, c.block * (BLOCK / 4) + threadIdx.x, (uint32_t)t, make_uint2((uint32_t)a.seed, (uint32_t)(a.seed >> 32)));
+        else f.update(h);
+        f.store(c, i, here);
+    };
+    if (c.count == CHUNK) chunk(4);           // no lane looks for an end
+    else chunk(c.count - i);
 }
 
 __global__ void adamw_count_kernel(float* step, const float* norm, const uint32_t* status) {
@@ -327,39 +389,66 @@ __device__ __forceinline__ double wave_sum(double x) {
     for (int d = 32; d > 0; d >>= 1) x += __shfl_xor(x, d, 64);
     return x;
 }
+// Chunks that a workgroup reads at a time, and most workgroups.  Two networks of 1.2 M weights: 4.1 us with 8, 4.9 with 16; 262 M bfloat16
+// gradients, past the caches: 85 us with 8 and 2048 workgroups, 80 us (6.6 TB/s) with 16 and 1024.
+constexpr int NORM_THREADS = 256;
+constexpr int norm_batch(bool past) { return past ? 16 : 8; }
+constexpr int norm_most(bool past) { return past ? 1024 : 2048; }
 __device__ __forceinline__ double group_sum(double x) {       // over the workgroup, in thread 0
-    __shared__ double part[THREADS / 64];
+    __shared__ double part[NORM_THREADS / 64];
     x = wave_sum(x);
     if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = x;
     __syncthreads();
     double s = 0.0;
-    for (int w = 0; w < THREADS / 64; ++w) s += part[w];
+    for (int w = 0; w < NORM_THREADS / 64; ++w) s += part[w];
     return s;
 }
 
 struct NormArgs {
-    const Entry* entries;
-    const int32_t* map;
-    int64_t chunk0, chunk1;
-    int32_t tensor0;
-    int32_t unroll;
+    const Chunk* chunks;
+    int64_t n_chunks;
+    int64_t tensor0;
     double* partials;        // one per workgroup
 };
-template <class GT, int N>
-__global__ __launch_bounds__(THREADS) void grad_norm_kernel(NormArgs a, Ptrs<N> grads) {
+// A workgroup takes BATCH chunks at a time.  Where they are one piece of one tensor - nearly always in a long list - their first
+// record says all, and FOURS loads of every thread are on their way together.
+template <class GT, int N, bool PAST>
+__global__ __launch_bounds__(NORM_THREADS) void grad_norm_kernel(NormArgs a, Ptrs<N> grads) {
+    constexpr int BATCH = norm_batch(PAST), FOURS = BATCH * CHUNK / 4 / NORM_THREADS;
+    auto address = [&](const Chunk& c) {
+        const char* gp = static_cast<const char*>(grads.p[c.tensor - a.tensor0]);
+        return gp ? gp + (int64_t)c.index * CHUNK * GT::BYTES : nullptr;
+    };
     double acc = 0.0;
-    for (int64_t chunk = a.chunk0 + blockIdx.x; chunk < a.chunk1; chunk += gridDim.x) {
-        const int tensor = a.map[chunk];
-        const void* gp = grads.p[tensor - a.tensor0];
-        if (!gp) continue;
-        const int64_t n = a.entries[tensor].n;
-        const int64_t base = (chunk - a.entries[tensor].first_chunk) * ((int64_t)THREADS * 4 * a.unroll);
-        for (int s = 0; s < a.unroll; ++s) {
-            const int64_t i = base + (int64_t)(s * THREADS + threadIdx.x) * 4;
-            const int64_t left = n - i;
-            if (left <= 0) break;
-            const float4v g = GT::widen(left >= 4 ? GT::load(gp, i) : GT::load_part(gp, i, (int)left));
-            for (int j = 0; j < 4; ++j) acc += (double)g[j] * (double)g[j];
+    auto add = [&](typename GT::raw g) {
+        const float4v x = GT::widen(g);
+        for (int j = 0; j < 4; ++j) acc = __builtin_fma((double)x[j], (double)x[j], acc);
+    };
+    for (int64_t k = (int64_t)blockIdx.x * BATCH; k < a.n_chunks; k += (int64_t)gridDim.x * BATCH) {
+        const int here = a.n_chunks - k < BATCH ? (int)(a.n_chunks - k) : BATCH;
+        const Chunk &c = a.chunks[k], &d = a.chunks[k + here - 1];
+        if (here == BATCH && c.tensor == d.tensor && d.count == CHUNK) {
+            const char* gp = address(c);
+            if (!gp) continue;
+            typename GT::raw g[FOURS];
+#pragma unroll
+            for (int s = 0; s < FOURS; ++s) g[s] = GT::template load<PAST>(gp, (s * NORM_THREADS + threadIdx.x) * 4, 4);
+#pragma unroll
+            for (int s = 0; s < FOURS; ++s) add(g[s]);
+        } else {
+            constexpr int SIDE = NORM_THREADS / THREADS;             // chunks side by side in the workgroup, whole wavefronts each
+            const int mine = __builtin_amdgcn_readfirstlane(threadIdx.x / THREADS), i = (threadIdx.x % THREADS) * 4;
+            typename GT::raw g[BATCH / SIDE];
+#pragma unroll
+            for (int b = 0; b < BATCH / SIDE; ++b) {
+                g[b] = 0;
+                if (b * SIDE + mine >= here) continue;
+                const Chunk& e = a.chunks[k + b * SIDE + mine];
+                const char* gp = address(e);
+                if (gp) g[b] = GT::template load<PAST>(gp, i, e.count - i);
+            }
+#pragma unroll
+            for (int b = 0; b < BATCH / SIDE; ++b) add(g[b]);
         }
     }
     const double s = group_sum(acc);
@@ -372,10 +461,10 @@ struct Counters {
     int n;
 };
 // words: [norm, coef, skip, skipped so far]; accumulate: the last one goes on counting
-__global__ __launch_bounds__(THREADS) void grad_norm_finish_kernel(const double* partials, int n, double max_norm, double grad_scale, float* words, int accumulate,
+__global__ __launch_bounds__(NORM_THREADS) void grad_norm_finish_kernel(const double* partials, int n, double max_norm, double grad_scale, float* words, int accumulate,
                                                                    const uint32_t* status, Counters counters) {
     double acc = 0.0;
-    for (int k = threadIdx.x; k < n; k += THREADS) acc += partials[k];
+    for (int k = threadIdx.x; k < n; k += NORM_THREADS) acc += partials[k];
     const double s = group_sum(acc);
     if (threadIdx.x != 0) return;
     const float norm = (float)(fabs(grad_scale) * sqrt(s));
@@ -390,6 +479,24 @@ __global__ __launch_bounds__(THREADS) void grad_norm_finish_kernel(const double*
 }
 
 // ---- host ------------------------------------------------------------------------------------------------------------------
+// of a list: SHORT, or MANY where a launch of the small kind cannot carry its addresses; PAST: more than the memory-side cache holds from
+// one step to the next, so it is read and written past the caches
+enum Shape { SHORT, MANY, PAST };
+int type_bytes(int type) { return type == BENERF_F32 ? 4 : 2; }
+int per_launch(int shape) { return shape == SHORT ? PTRS_SMALL : PTRS_LARGE; }
+int64_t count_chunks(const BenerfAdamwTensor* t, int n) {
+    int64_t chunks = 0;
+    for (int k = 0; k < n; ++k) chunks += (t[k].n + CHUNK - 1) / CHUNK;
+    return chunks;
+}
+int plan_shape(const BenerfAdamwTensor* t, int n, int param_type, int state_bits) {
+    int64_t total = 0;
+    for (int k = 0; k < n; ++k) total += t[k].n;
+    const int width = type_bytes(param_type);
+    const int64_t bytes = total * (state_bits == 0 ? width : 2 * width + (state_bits == 8 ? 2 : 8) + (n > 0 && t[0].master ? 4 : 0));
+    return bytes > PAST_BYTES ? PAST : n <= PTRS_SMALL ? SHORT : MANY;
+}
+
 bool plan_ok(const PlanHead* p) { return p && p->magic == PLAN_MAGIC && p->n_tensors > 0; }
 
 // tensors per launch, and one launch per run of tensors that holds a gradient
@@ -397,7 +504,7 @@ template <class F>
 int for_launches(const void* plan_host, const void* const* grads_host, F&& launch) {
     const PlanHead* h = static_cast<const PlanHead*>(plan_host);
     const Entry* e = plan_entries(plan_host);
-    const int per = h->n_tensors <= PTRS_SMALL ? PTRS_SMALL : PTRS_LARGE;
+    const int per = per_launch(h->shape);
     for (int t0 = 0; t0 < h->n_tensors; t0 += per) {
         int lo = t0, hi = t0 + per < h->n_tensors ? t0 + per : h->n_tensors;
         while (lo < hi && (!grads_host[lo] || e[lo].n == 0)) ++lo;
@@ -410,63 +517,66 @@ int for_launches(const void* plan_host, const void* const* grads_host, F&& launc
     return BENERF_OK;
 }
 
-template <class PT, class GT, int BITS, bool MASTER, int N>
-void launch_adamw(const AdamwArgs& a, int64_t chunks, const void* const* grads, int count, hipStream_t s) {
+template <int N>
+Ptrs<N> pack(const void* const* grads, int count) {
     Ptrs<N> p;
     for (int k = 0; k < N; ++k) p.p[k] = k < count ? grads[k] : nullptr;
-    hipLaunchKernelGGL((adamw_kernel<PT, GT, BITS, MASTER, N>), dim3((unsigned)chunks), dim3(THREADS), 0, s, a, p);
+    return p;
 }
 typedef void (*AdamwLaunch)(const AdamwArgs&, int64_t, const void* const*, int, hipStream_t);
+template <class PT, class GT, int BITS, bool MASTER, int N, bool PAST>
+void launch_adamw(const AdamwArgs& a, int64_t chunks, const void* const* grads, int count, hipStream_t s) {
+    hipLaunchKernelGGL((adamw_kernel<PT, GT, BITS, MASTER, N, PAST>), dim3((unsigned)chunks), dim3(THREADS), 0, s, a, pack<N>(grads, count));
+}
 template <class PT, class GT, int BITS, bool MASTER>
-AdamwLaunch by_count(bool small) {
-    return small ? launch_adamw<PT, GT, BITS, MASTER, PTRS_SMALL> : launch_adamw<PT, GT, BITS, MASTER, PTRS_LARGE>;
+AdamwLaunch by_shape(int shape) {
+    switch (shape) {
+        case SHORT: return launch_adamw<PT, GT, BITS, MASTER, PTRS_SMALL, false>;
+        case MANY: return launch_adamw<PT, GT, BITS, MASTER, PTRS_LARGE, false>;
+        default: return launch_adamw<PT, GT, BITS, MASTER, PTRS_LARGE, true>;
+    }
 }
 template <class PT, class GT>
-AdamwLaunch by_state(int bits, bool master, bool small) {
-    if constexpr (!PT::NARROW) return bits == 8 ? by_count<PT, GT, 8, false>(small) : by_count<PT, GT, 32, false>(small);      // f32 is its own master
-    else if (bits == 8) return master ? by_count<PT, GT, 8, true>(small) : by_count<PT, GT, 8, false>(small);
-    else return master ? by_count<PT, GT, 32, true>(small) : by_count<PT, GT, 32, false>(small);
+AdamwLaunch by_state(int bits, bool master, int shape) {
+    if constexpr (!PT::NARROW) return bits == 8 ? by_shape<PT, GT, 8, false>(shape) : by_shape<PT, GT, 32, false>(shape);      // f32 is its own master
+    else if (bits == 8) return master ? by_shape<PT, GT, 8, true>(shape) : by_shape<PT, GT, 8, false>(shape);
+    else return master ? by_shape<PT, GT, 32, true>(shape) : by_shape<PT, GT, 32, false>(shape);
 }
 template <class PT>
-AdamwLaunch by_grad(int grad_type, int bits, bool master, bool small) {
+AdamwLaunch by_grad(int grad_type, int bits, bool master, int shape) {
     switch (grad_type) {
-        case BENERF_F32: return by_state<PT, F32>(bits, master, small);
-        case BENERF_BF16: return by_state<PT, BF16>(bits, master, small);
-        default: return by_state<PT, F16>(bits, master, small);
+        case BENERF_F32: return by_state<PT, F32>(bits, master, shape);
+        case BENERF_BF16: return by_state<PT, BF16>(bits, master, shape);
+        default: return by_state<PT, F16>(bits, master, shape);
     }
 }
 
-template <class GT, int N>
+typedef void (*NormLaunch)(const NormArgs&, int, const void* const*, int, hipStream_t);
+template <class GT, int N, bool PAST>
 void launch_norm(const NormArgs& a, int blocks, const void* const* grads, int count, hipStream_t s) {
-    Ptrs<N> p;
-    for (int k = 0; k < N; ++k) p.p[k] = k < count ? grads[k] : nullptr;
-    hipLaunchKernelGGL((grad_norm_kernel<GT, N>), dim3((unsigned)blocks), dim3(THREADS), 0, s, a, p);
+    hipLaunchKernelGGL((grad_norm_kernel<GT, N, PAST>), dim3((unsigned)blocks), dim3(NORM_THREADS), 0, s, a, pack<N>(grads, count));
+}
+template <class GT>
+NormLaunch norm_by_shape(int shape) {
+    switch (shape) {
+        case SHORT: return launch_norm<GT, PTRS_SMALL, false>;
+        case MANY: return launch_norm<GT, PTRS_LARGE, false>;
+        default: return launch_norm<GT, PTRS_LARGE, true>;
+    }
 }
 
-int type_bytes(int type) { return type == BENERF_F32 ? 4 : 2; }
-int norm_blocks(int64_t chunks) { return (int)(chunks < 1024 ? chunks : 1024); }
+int norm_blocks(int64_t chunks, int shape) {
+    const int64_t batch = norm_batch(shape == PAST), most = norm_most(shape == PAST), blocks = (chunks + batch - 1) / batch;
+    return (int)(blocks < most ? blocks : most);
+}
 
 }  // namespace
-
-// A chunk of 4096 elements keeps four independent loads of every array in flight; lists too short to give every CU two of them are cut
-// into chunks of 1024.
-static int plan_unroll(const BenerfAdamwTensor* t, int n) {
-    int64_t chunks = 0;
-    for (int k = 0; k < n; ++k) chunks += (t[k].n + 4 * 4 * THREADS - 1) / (4 * 4 * THREADS);
-    return chunks >= 512 ? 4 : 1;
-}
-static int64_t plan_chunks(const BenerfAdamwTensor* t, int n, int unroll) {
-    const int64_t size = (int64_t)THREADS * 4 * unroll;
-    int64_t chunks = 0;
-    for (int k = 0; k < n; ++k) chunks += (t[k].n + size - 1) / size;
-    return chunks;
-}
 
 extern "C" size_t benerf_adamw_plan_bytes(const BenerfAdamwTensor* tensors_host, int n_tensors) {
     if (!tensors_host || n_tensors <= 0) return 0;
     for (int k = 0; k < n_tensors; ++k)
         if (tensors_host[k].n < 0 || tensors_host[k].n > (1ll << 40)) return 0;
-    return HEAD_BYTES + sizeof(Entry) * (size_t)n_tensors + 4 * (size_t)plan_chunks(tensors_host, n_tensors, plan_unroll(tensors_host, n_tensors));
+    return HEAD_BYTES + sizeof(Entry) * (size_t)n_tensors + sizeof(Chunk) * (size_t)count_chunks(tensors_host, n_tensors);
 }
 
 extern "C" int benerf_adamw_plan_fill(const BenerfAdamwTensor* tensors_host, int n_tensors, int param_type, int state_bits, void* plan_host, size_t plan_bytes) {
@@ -500,19 +610,33 @@ extern "C" int benerf_adamw_plan_fill(const BenerfAdamwTensor* tensors_host, int
     h->param_type = param_type;
     h->state_bits = state_bits;
     h->has_master = master;
-    h->unroll = plan_unroll(tensors_host, n_tensors);
-    h->n_chunks = plan_chunks(tensors_host, n_tensors, h->unroll);
-    h->map_at = (int64_t)(HEAD_BYTES + sizeof(Entry) * (size_t)n_tensors);
+    h->shape = plan_shape(tensors_host, n_tensors, param_type, state_bits);
+    h->n_chunks = count_chunks(tensors_host, n_tensors);
+    h->chunks_at = (int64_t)(HEAD_BYTES + sizeof(Entry) * (size_t)n_tensors);
     h->bytes = (int64_t)need;
-    BENERF_REQUIRE(h->n_chunks < (1ll << 24), "adamw_plan_fill: more than 2^24 chunks of 4096 elements");      // a grid holds 2^32 threads
+    BENERF_REQUIRE(h->n_chunks < (1ll << 24), "adamw_plan_fill: more than 2^24 chunks of 512 elements");      // a grid holds 2^32 threads
     Entry* e = reinterpret_cast<Entry*>(static_cast<char*>(plan_host) + HEAD_BYTES);
-    int32_t* map = reinterpret_cast<int32_t*>(static_cast<char*>(plan_host) + h->map_at);
-    const int64_t size = (int64_t)THREADS * 4 * h->unroll;
-    int64_t chunk = 0;
+    Chunk* chunk = reinterpret_cast<Chunk*>(static_cast<char*>(plan_host) + h->chunks_at);
+    int64_t at = 0;
+    auto on = [](void* p, int64_t bytes) { return p ? static_cast<char*>(p) + bytes : nullptr; };
     for (int k = 0; k < n_tensors; ++k) {
         const BenerfAdamwTensor& t = tensors_host[k];
-        e[k] = Entry{t.param, t.exp_avg, t.exp_avg_sq, t.exp_avg_scale, t.exp_avg_sq_scale, t.master, t.n, t.first_block, chunk};
-        for (int64_t c = (t.n + size - 1) / size; c > 0; --c) map[chunk++] = k;
+        e[k] = Entry{t.n, at};
+        for (int64_t i = 0; i < t.n; i += CHUNK, ++at, ++chunk) {
+            const int64_t w = state_bits == 8 ? 1 : 4;
+            chunk->param = on(t.param, i * type_bytes(param_type));
+            chunk->m = on(t.exp_avg, i * w);
+            chunk->v = on(t.exp_avg_sq, i * w);
+            if (state_bits == 8) {
+                chunk->ms = t.exp_avg_scale + i / BLOCK;
+                chunk->vs = t.exp_avg_sq_scale + i / BLOCK;
+            }
+            chunk->master = t.master ? t.master + i : nullptr;
+            chunk->block = t.first_block + i / BLOCK;
+            chunk->tensor = k;
+            chunk->index = (int32_t)(i / CHUNK);
+            chunk->count = (int32_t)(t.n - i < CHUNK ? t.n - i : CHUNK);
+        }
     }
     return BENERF_OK;
 }
@@ -530,9 +654,6 @@ extern "C" int benerf_adamw_step(const void* plan_host, const void* plan_dev, co
         BENERF_REQUIRE(((uintptr_t)grads_host[k] & (uintptr_t)(type_bytes(grad_type) - 1)) == 0, "adamw_step: gradient %d is not aligned to its elements", k);
     AdamwArgs a;
     memset(&a, 0, sizeof(a));
-    a.entries = plan_entries(plan_dev);
-    a.map = reinterpret_cast<const int32_t*>(static_cast<const char*>(plan_dev) + ph->map_at);
-    a.unroll = ph->unroll;
     a.norm = norm_words;
     a.status = skip_if_range;
     a.step_dev = cfg->step_dev;
@@ -552,12 +673,11 @@ extern "C" int benerf_adamw_step(const void* plan_host, const void* plan_dev, co
     a.h.decay = (float)(1.0 - cfg->lr * cfg->weight_decay);
     a.h.step_size = (float)(cfg->lr / (1.0 - int_power(cfg->beta1, t)));
     a.h.inv_bc2 = (float)(1.0 / sqrt(1.0 - int_power(cfg->beta2, t)));
-    const bool small = ph->n_tensors <= PTRS_SMALL;
-    AdamwLaunch f = ph->param_type == BENERF_F32 ? by_grad<F32>(grad_type, ph->state_bits, ph->has_master, small)
-                    : ph->param_type == BENERF_BF16 ? by_grad<BF16>(grad_type, ph->state_bits, ph->has_master, small)
-                                                    : by_grad<F16>(grad_type, ph->state_bits, ph->has_master, small);
+    AdamwLaunch f = ph->param_type == BENERF_F32 ? by_grad<F32>(grad_type, ph->state_bits, ph->has_master, ph->shape)
+                    : ph->param_type == BENERF_BF16 ? by_grad<BF16>(grad_type, ph->state_bits, ph->has_master, ph->shape)
+                                                    : by_grad<F16>(grad_type, ph->state_bits, ph->has_master, ph->shape);
     return for_launches(plan_host, grads_host, [&](int lo, int count, int64_t c0, int64_t c1) -> int {
-        a.chunk0 = c0;
+        a.chunks = plan_chunks_dev(plan_dev, ph) + c0;
         a.tensor0 = lo;
         f(a, c1 - c0, grads_host + lo, count, as_stream(stream));
         BENERF_LAUNCH_CHECK("adamw_step");
@@ -575,8 +695,8 @@ extern "C" int benerf_adamw_count(float* step_dev, const float* norm_words, cons
 extern "C" size_t benerf_grad_norm_partials(const void* plan_host) {
     const PlanHead* ph = static_cast<const PlanHead*>(plan_host);
     if (!plan_ok(ph)) return 0;
-    const int per = ph->n_tensors <= PTRS_SMALL ? PTRS_SMALL : PTRS_LARGE;
-    return (size_t)norm_blocks(ph->n_chunks < 1 ? 1 : ph->n_chunks) * (size_t)((ph->n_tensors + per - 1) / per);
+    const int per = per_launch(ph->shape);
+    return (size_t)norm_blocks(ph->n_chunks < 1 ? 1 : ph->n_chunks, ph->shape) * (size_t)((ph->n_tensors + per - 1) / per);
 }
 
 extern "C" int benerf_grad_norm_partial(const void* plan_host, const void* plan_dev, const void* const* grads_host, int grad_type, double* partials, size_t n_partials,
@@ -587,27 +707,20 @@ extern "C" int benerf_grad_norm_partial(const void* plan_host, const void* plan_
     for (int k = 0; k < ph->n_tensors; ++k)
         BENERF_REQUIRE(((uintptr_t)grads_host[k] & (uintptr_t)(type_bytes(grad_type) - 1)) == 0, "grad_norm_partial: gradient %d is not aligned to its elements", k);
     NormArgs a;
-    a.entries = plan_entries(plan_dev);
-    a.map = reinterpret_cast<const int32_t*>(static_cast<const char*>(plan_dev) + ph->map_at);
-    a.unroll = ph->unroll;
-    const bool small = ph->n_tensors <= PTRS_SMALL;
+    const NormLaunch f = grad_type == BENERF_F32 ? norm_by_shape<F32>(ph->shape) : grad_type == BENERF_BF16 ? norm_by_shape<BF16>(ph->shape) : norm_by_shape<F16>(ph->shape);
     int64_t used = 0;
     const int rc = for_launches(plan_host, grads_host, [&](int lo, int count, int64_t c0, int64_t c1) -> int {
-        const int blocks = norm_blocks(c1 - c0);
+        const int blocks = norm_blocks(c1 - c0, ph->shape);
         if ((size_t)(used + blocks) > n_partials) {
             benerf_set_error("grad_norm_partial: room for %zu partial sums, benerf_grad_norm_partials says how many", n_partials);
             return BENERF_EWORKSPACE;
         }
-        a.chunk0 = c0;
-        a.chunk1 = c1;
+        a.chunks = plan_chunks_dev(plan_dev, ph) + c0;
+        a.n_chunks = c1 - c0;
         a.tensor0 = lo;
         a.partials = partials + used;
         used += blocks;
-        const void* const* g = grads_host + lo;
-        hipStream_t s = as_stream(stream);
-        if (grad_type == BENERF_F32) small ? launch_norm<F32, PTRS_SMALL>(a, blocks, g, count, s) : launch_norm<F32, PTRS_LARGE>(a, blocks, g, count, s);
-        else if (grad_type == BENERF_BF16) small ? launch_norm<BF16, PTRS_SMALL>(a, blocks, g, count, s) : launch_norm<BF16, PTRS_LARGE>(a, blocks, g, count, s);
-        else small ? launch_norm<F16, PTRS_SMALL>(a, blocks, g, count, s) : launch_norm<F16, PTRS_LARGE>(a, blocks, g, count, s);
+        f(a, blocks, grads_host + lo, count, as_stream(stream));
         BENERF_LAUNCH_CHECK("grad_norm_partial");
         return BENERF_OK;
     });
@@ -627,7 +740,7 @@ extern "C" int benerf_grad_norm_finish(const double* partials, int64_t n_partial
         BENERF_REQUIRE(counters_host[k], "grad_norm_finish: null counter");
         c.p[k] = counters_host[k];
     }
-    hipLaunchKernelGGL(grad_norm_finish_kernel, dim3(1), dim3(THREADS), 0, as_stream(stream), partials, (int)n_partials, max_norm, grad_scale, words, accumulate,
+    hipLaunchKernelGGL(grad_norm_finish_kernel, dim3(1), dim3(NORM_THREADS), 0, as_stream(stream), partials, (int)n_partials, max_norm, grad_scale, words, accumulate,
                        skip_if_range, c);
     BENERF_LAUNCH_CHECK("grad_norm_finish");
     return BENERF_OK;

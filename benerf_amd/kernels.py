@@ -771,7 +771,8 @@ class GradList:
         if plan is not None:
             self.parts = plan.parts
         else:
-            self.parts = [_Part(range(len(tensors)), [_lib.AdamwTensor(n=0 if t is None else t.numel()) for t in self.tensors], 0, 0, self.device)]
+            kind = next(t.dtype for t in self.tensors if t is not None)
+            self.parts = [_Part(range(len(tensors)), [_lib.AdamwTensor(n=0 if t is None else t.numel()) for t in self.tensors], _ELEMENT_TYPES[kind], 0, self.device)]
         self.launches = _grad_launches(self.parts, self.tensors)
 
     @classmethod

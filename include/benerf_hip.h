@@ -411,7 +411,7 @@ int benerf_adam_step(float* param, const float* grad, float* exp_avg, float* exp
  *   state_bits 32: exp_avg, exp_avg_sq float32 [n], the scale pointers are not read;
  *   state_bits 8:  exp_avg uint8 [n] e4m3 codes of m, exp_avg_sq uint8 [n] e4m3 codes of sqrt(v), *_scale float32 [ceil(n / 128)]: the
  *                  power of two that belongs to 128 consecutive elements (0 moments: any scale with codes 0);
- *   state_bits 0:  a plan for benerf_grad_norm_partial alone, only n is read.
+ *   state_bits 0:  a plan for benerf_grad_norm_partial alone, only n is read (param_type: the gradients').
  *   master: float32 [n], or NULL: the parameter itself is read.  With it, param is written only.
  *   first_block: number of the tensor's first block of 128 in the caller's numbering (8 bits: the generator's counter; give every
  *                tensor its own range).

@@ -29,12 +29,10 @@ def _fill(lib, rows, kind=0, bits=32, short=0):
 
 
 def test_plan_sizes(lib):
-    # header 64, 72 bytes a tensor, 4 bytes a chunk: 1024 elements a chunk in a short list, 4096 from 512 chunks of that size on
-    assert lib.benerf_adamw_plan_bytes(_rows(1), 1) == 64 + 72 + 4
-    assert lib.benerf_adamw_plan_bytes(_rows(1024, 1025, 0), 3) == 64 + 3 * 72 + 4 * 3
-    assert lib.benerf_adamw_plan_bytes(_rows(512 * 4096), 1) == 64 + 72 + 4 * 512
-    assert lib.benerf_adamw_plan_bytes(_rows(-1), 1) == 0 and lib.benerf_adamw_plan_bytes(_rows(1 << 41), 1) == 0
-    assert lib.benerf_adamw_plan_bytes(None, 1) == 0
+    # header 64, 16 bytes a tensor, 80 bytes a chunk of 512 elements
+    size = lambda *ns: lib.benerf_adamw_plan_bytes(_rows(*ns), len(ns))      # noqa: E731
+    assert size(1) == 64 + 16 + 80 and size(512, 513, 0) == 64 + 3 * 16 + 80 * 3 and size(1 << 30) == 64 + 16 + (80 << 21)
+    assert size(-1) == 0 and size(1 << 41) == 0 and lib.benerf_adamw_plan_bytes(None, 1) == 0
 
 
 def test_plan_refusals(lib):
