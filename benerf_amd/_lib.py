@@ -39,6 +39,10 @@ class AdamwTensor(Structure):
                 ("master", c_void_p), ("n", c_int64), ("first_block", c_int64)]
 
 
+class GradListRow(Structure):
+    _fields_ = [("plan_host", c_void_p), ("plan_dev", c_void_p), ("grads_host", c_void_p), ("grad_type", c_int32)]
+
+
 class AdamwCfg(Structure):
     _fields_ = [("lr", c_double), ("beta1", c_double), ("beta2", c_double), ("eps", c_double), ("weight_decay", c_double), ("grad_scale", c_double),
                 ("step", c_int64), ("seed", c_uint64), ("lr_dev", c_void_p), ("step_dev", c_void_p)]
@@ -102,8 +106,7 @@ _SIGNATURES = {
     "benerf_adamw_step": (c_int, [P, P, P, c_int, POINTER(AdamwCfg), P, P, P]),
     "benerf_adamw_count": (c_int, [P, P, P, P]),
     "benerf_grad_norm_partials": (c_size_t, [P]),
-    "benerf_grad_norm_partial": (c_int, [P, P, P, c_int, P, c_size_t, POINTER(c_int64), P]),
-    "benerf_grad_norm_finish": (c_int, [P, c_int64, c_double, c_double, P, c_int, P, P, c_int, P]),
+    "benerf_grad_norm": (c_int, [P, c_int, P, c_size_t, c_double, c_double, P, c_int, P, P, c_int, P]),
 }
 
 EXPORTED_SYMBOLS = tuple(sorted(_SIGNATURES))

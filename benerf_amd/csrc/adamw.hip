@@ -699,49 +699,50 @@ extern "C" size_t benerf_grad_norm_partials(const void* plan_host) {
     return (size_t)norm_blocks(ph->n_chunks < 1 ? 1 : ph->n_chunks, ph->shape) * (size_t)((ph->n_tensors + per - 1) / per);
 }
 
-extern "C" int benerf_grad_norm_partial(const void* plan_host, const void* plan_dev, const void* const* grads_host, int grad_type, double* partials, size_t n_partials,
-                                        int64_t* used_host, benerf_stream_t stream) {
-    const PlanHead* ph = static_cast<const PlanHead*>(plan_host);
-    BENERF_REQUIRE(plan_ok(ph) && plan_dev && grads_host && partials && used_host, "grad_norm_partial: null pointer, or no plan");
-    BENERF_REQUIRE(grad_type >= BENERF_F32 && grad_type <= BENERF_F16, "grad_norm_partial: unknown gradient type %d", grad_type);
-    for (int k = 0; k < ph->n_tensors; ++k)
-        BENERF_REQUIRE(((uintptr_t)grads_host[k] & (uintptr_t)(type_bytes(grad_type) - 1)) == 0, "grad_norm_partial: gradient %d is not aligned to its elements", k);
-    NormArgs a;
-    const NormLaunch f = grad_type == BENERF_F32 ? norm_by_shape<F32>(ph->shape) : grad_type == BENERF_BF16 ? norm_by_shape<BF16>(ph->shape) : norm_by_shape<F16>(ph->shape);
-    int64_t used = 0;
-    const int rc = for_launches(plan_host, grads_host, [&](int lo, int count, int64_t c0, int64_t c1) -> int {
-        const int blocks = norm_blocks(c1 - c0, ph->shape);
-        if ((size_t)(used + blocks) > n_partials) {
-            benerf_set_error("grad_norm_partial: room for %zu partial sums, benerf_grad_norm_partials says how many", n_partials);
-            return BENERF_EWORKSPACE;
-        }
-        a.chunks = plan_chunks_dev(plan_dev, ph) + c0;
-        a.n_chunks = c1 - c0;
-        a.tensor0 = lo;
-        a.partials = partials + used;
-        used += blocks;
-        f(a, blocks, grads_host + lo, count, as_stream(stream));
-        BENERF_LAUNCH_CHECK("grad_norm_partial");
-        return BENERF_OK;
-    });
-    *used_host = used;
-    return rc;
-}
-
-extern "C" int benerf_grad_norm_finish(const double* partials, int64_t n_partials, double max_norm, double grad_scale, float* words, int accumulate,
-                                       const uint32_t* skip_if_range, float* const* counters_host, int n_counters, benerf_stream_t stream) {
-    BENERF_REQUIRE(words && (partials || n_partials == 0) && n_partials >= 0 && n_partials < (1ll << 31), "grad_norm_finish: bad args");
-    BENERF_REQUIRE(max_norm > 0.0, "grad_norm_finish: max_norm must be positive (infinity: no clipping)");
-    BENERF_REQUIRE(n_counters >= 0 && n_counters <= MAX_COUNTERS && (counters_host || n_counters == 0), "grad_norm_finish: at most %d counters", MAX_COUNTERS);
+extern "C" int benerf_grad_norm(const BenerfGradList* lists_host, int n_lists, double* partials, size_t n_partials, double max_norm, double grad_scale, float* words,
+                                int accumulate, const uint32_t* skip_if_range, float* const* counters_host, int n_counters, benerf_stream_t stream) {
+    BENERF_REQUIRE((lists_host || n_lists == 0) && n_lists >= 0 && words, "grad_norm: null pointer");
+    BENERF_REQUIRE(max_norm > 0.0, "grad_norm: max_norm must be positive (infinity: no clipping)");
+    BENERF_REQUIRE(n_counters >= 0 && n_counters <= MAX_COUNTERS && (counters_host || n_counters == 0), "grad_norm: at most %d counters", MAX_COUNTERS);
     Counters c;
     memset(&c, 0, sizeof(c));
     c.n = n_counters;
     for (int k = 0; k < n_counters; ++k) {
-        BENERF_REQUIRE(counters_host[k], "grad_norm_finish: null counter");
+        BENERF_REQUIRE(counters_host[k], "grad_norm: null counter");
         c.p[k] = counters_host[k];
     }
-    hipLaunchKernelGGL(grad_norm_finish_kernel, dim3(1), dim3(NORM_THREADS), 0, as_stream(stream), partials, (int)n_partials, max_norm, grad_scale, words, accumulate,
-                       skip_if_range, c);
-    BENERF_LAUNCH_CHECK("grad_norm_finish");
+    size_t room = 0;
+    for (int l = 0; l < n_lists; ++l) {
+        const BenerfGradList& g = lists_host[l];
+        const PlanHead* ph = static_cast<const PlanHead*>(g.plan_host);
+        BENERF_REQUIRE(plan_ok(ph) && g.plan_dev && g.grads_host, "grad_norm: list %d: null pointer, or no plan", l);
+        BENERF_REQUIRE(g.grad_type >= BENERF_F32 && g.grad_type <= BENERF_F16, "grad_norm: list %d: unknown gradient type %d", l, g.grad_type);
+        for (int k = 0; k < ph->n_tensors; ++k)
+            BENERF_REQUIRE(((uintptr_t)g.grads_host[k] & (uintptr_t)(type_bytes(g.grad_type) - 1)) == 0, "grad_norm: gradient %d is not aligned to its elements", k);
+        room += benerf_grad_norm_partials(g.plan_host);
+    }
+    BENERF_REQUIRE(room < (1ull << 31) && (partials || room == 0), "grad_norm: null pointer");
+    if (n_partials < room) {
+        benerf_set_error("grad_norm: room for %zu partial sums, %zu needed (benerf_grad_norm_partials of every list)", n_partials, room);
+        return BENERF_EWORKSPACE;
+    }
+    hipStream_t s = as_stream(stream);
+    int used = 0;
+    for (int l = 0; l < n_lists; ++l) {
+        const BenerfGradList& g = lists_host[l];
+        const PlanHead* ph = static_cast<const PlanHead*>(g.plan_host);
+        const NormLaunch f = g.grad_type == BENERF_F32 ? norm_by_shape<F32>(ph->shape) : g.grad_type == BENERF_BF16 ? norm_by_shape<BF16>(ph->shape) : norm_by_shape<F16>(ph->shape);
+        const int rc = for_launches(g.plan_host, g.grads_host, [&](int lo, int count, int64_t c0, int64_t c1) -> int {
+            const int blocks = norm_blocks(c1 - c0, ph->shape);
+            const NormArgs a = {plan_chunks_dev(g.plan_dev, ph) + c0, c1 - c0, lo, partials + used};
+            used += blocks;
+            f(a, blocks, g.grads_host + lo, count, s);
+            BENERF_LAUNCH_CHECK("grad_norm");
+            return BENERF_OK;
+        });
+        if (rc != BENERF_OK) return rc;
+    }
+    hipLaunchKernelGGL(grad_norm_finish_kernel, dim3(1), dim3(NORM_THREADS), 0, s, partials, used, max_norm, grad_scale, words, accumulate, skip_if_range, c);
+    BENERF_LAUNCH_CHECK("grad_norm");
     return BENERF_OK;
 }

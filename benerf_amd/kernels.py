@@ -2,6 +2,7 @@
 include/benerf_hip.h).  PyTorch is plumbing only: device memory, streams, autograd glue.
 Every wrapper validates dtype / device / contiguity and raises on any non-zero return code.
 """
+import array
 import ctypes
 import os
 
@@ -691,22 +692,6 @@ _ELEMENT_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 CODE_TYPE = torch.float8_e4m3fn     # 8-bit moments: a code is an e4m3 number, its value the number times its block's scale
 
 
-def _on(device):
-    """Context that makes `device` the current one (launches go to ITS current stream); free of charge where it already is."""
-    return _NOTHING if _cur_device is not None and device.index == _cur_device() else torch.cuda.device(device)
-
-
-class _Nothing:
-    def __enter__(self):
-        return None
-
-    def __exit__(self, *exc):
-        return False
-
-
-_NOTHING = _Nothing()
-
-
 def _list_tensor(t, name, device, dtypes, numel=None):
     """Checks one tensor of a list and returns an alias of it that keeps its memory alive whatever the caller does to `t`."""
     if not torch.is_tensor(t):
@@ -740,17 +725,17 @@ class _Part:
         self.host = ctypes.create_string_buffer(size)
         _lib.check(lib.benerf_adamw_plan_fill(table, n, param_type, state_bits, self.host, size), "adamw_plan_fill")
         self.state_bits = state_bits
-        with _on(device):
+        with torch.cuda.device(device):
             # a blocking copy: the plan is there before anything is queued on any stream
             self.dev = torch.frombuffer(bytearray(self.host.raw), dtype=torch.uint8).to(device)
             self.stream = _stream()
-            self.partials = int(lib.benerf_grad_norm_partials(self.host))
+        self.host_at, self.dev_at = ctypes.addressof(self.host), self.dev.data_ptr()
+        self.partials = int(lib.benerf_grad_norm_partials(self.host))
 
-    def on_device(self):
-        """Address of the device copy for a launch on the current stream."""
-        if _stream() != self.stream:
+    def used_on(self, stream):
+        """A launch on `stream` reads the device copy: it must outlive it."""
+        if stream != self.stream:
             self.dev.record_stream(torch.cuda.current_stream(self.dev.device))
-        return self.dev.data_ptr()
 
 
 class GradList:
@@ -773,30 +758,34 @@ class GradList:
         else:
             kind = next(t.dtype for t in self.tensors if t is not None)
             self.parts = [_Part(range(len(tensors)), [_lib.AdamwTensor(n=0 if t is None else t.numel()) for t in self.tensors], _ELEMENT_TYPES[kind], 0, self.device)]
-        self.launches = _grad_launches(self.parts, self.tensors)
+        self._bind()
 
     @classmethod
     def of_checked(cls, tensors, plan):
-        """The gradients of a plan's own parameters (contiguous; torch holds their sizes and devices to the parameters'): no checks."""
+        """The gradients of a plan's own parameters, contiguous and of their sizes: no checks."""
         self = cls.__new__(cls)
         self.device, self.tensors, self.parts = plan.device, tensors, plan.parts
-        self.launches = _grad_launches(plan.parts, tensors)
+        self._bind()
         return self
+
+    def _bind(self):
+        self.launches = launches = _grad_launches(self.parts, self.tensors)
+        self.rows = (_lib.GradListRow * len(launches))(*[(p.host_at, p.dev_at, a.buffer_info()[0], kind) for p, kind, a in launches])
+        self.room = sum(p.partials for p, _, _ in launches)
 
 
 def _grad_launches(parts, tensors):
     """[(part, element type, array of device addresses)]: one launch sequence for every type of gradient in every part."""
     out = []
     for part in parts:
-        by_type = {}
-        for k, i in enumerate(part.index):
-            t = tensors[i]
-            if t is not None:
-                a = by_type.get(t.dtype)
-                if a is None:
-                    a = by_type[t.dtype] = (ctypes.c_void_p * part.count)()
-                a[k] = t.data_ptr()
-        out += [(part, _ELEMENT_TYPES[d], a) for d, a in by_type.items()]
+        mine = tensors if part.count == len(tensors) else [tensors[i] for i in part.index]
+        kinds = [None if t is None else t.dtype for t in mine]
+        if kinds.count(kinds[0]) == len(kinds):
+            if kinds[0] is not None:
+                out.append((part, _ELEMENT_TYPES[kinds[0]], array.array("Q", [t.data_ptr() for t in mine])))
+        else:
+            for kind in {k: None for k in kinds if k is not None}:
+                out.append((part, _ELEMENT_TYPES[kind], array.array("Q", [t.data_ptr() if k is kind else 0 for t, k in zip(mine, kinds)])))
     return out
 
 
@@ -857,7 +846,7 @@ class AdamWPlan:
                     self.master.append(None)
                 else:
                     self.master.append(_list_tensor(t, "master %d" % k, self.device, (torch.float32,), self.numels[k]))
-        mlp_status(self.device)             # the guard's words exist (and are zero) before a step can be captured
+        self.guard = mlp_status(self.device).data_ptr()       # the guard's words exist (and are zero) before a step can be captured
         _no_overlap([self.params, self.exp_avg, self.exp_avg_sq, self.exp_avg_scale, self.exp_avg_sq_scale, self.master])
         at = lambda l, k: None if l is None or l[k] is None else l[k].data_ptr()       # noqa: E731
         rows, block = {}, 0
@@ -880,8 +869,16 @@ def _as_grads(grads, plan=None):
     return grads
 
 
-def _guard_words(device, guard_range, status):
-    return (mlp_status(device) if status is None else status).data_ptr() if guard_range else None
+def _counter(t, device):
+    if t.numel() != 1 or t.device != device:
+        raise ValueError("a counter or rate on the device is one float32 on %s" % device)
+    return _chk(t, name="counter")
+
+
+def _norm_words(t, device, name):
+    if t.numel() != 4 or t.device != device:
+        raise ValueError("%s: the 4 words of a norm on %s" % (name, device))
+    return _chk(t, name=name)
 
 
 def grad_norm(grads, max_norm=float("inf"), grad_scale=1.0, out=None, counters=(), guard_range=False, status=None):
@@ -889,47 +886,46 @@ def grad_norm(grads, max_norm=float("inf"), grad_scale=1.0, out=None, counters=(
     device and without synchronising.  Returns float32 [4] = [norm of grad_scale * gradients, coefficient min(1, max_norm / (norm +
     1e-6)), 1 if the step must be skipped (norm not finite, or guard_range and the range guard's words say so), skipped steps so far];
     hand it to `adamw_step(norm=...)`.  out: such a tensor (zeroed once by the caller) to write, whose count of skipped steps goes on.
-    counters: float32 1-element step counters on the device that go up by one unless the step is skipped."""
-    lib = _lib.load()
+    counters: up to 64 float32 1-element step counters on the device that go up by one unless the step is skipped."""
     if not max_norm > 0:
         raise ValueError("grad_norm: max_norm must be positive, got %r" % (max_norm,))
-    lists = [grads] if isinstance(grads, GradList) else list(grads)
-    lists = [g if isinstance(g, GradList) else _as_grads(g) for g in (lists if lists and isinstance(lists[0], GradList) else [lists])]
+    if isinstance(grads, GradList):
+        rows, room, lists = grads.rows, grads.room, (grads,)
+    else:
+        lists = list(grads)
+        if not lists or not isinstance(lists[0], GradList):
+            lists = [GradList(lists)]
+        if any(g.device != lists[0].device for g in lists):
+            raise ValueError("grad_norm: gradients on several devices")
+        rows = (_lib.GradListRow * sum(len(g.rows) for g in lists))(*[r for g in lists for r in g.rows])
+        room = sum(g.room for g in lists)
     dev = lists[0].device
-    if any(g.device != dev for g in lists):
-        raise ValueError("grad_norm: gradients on several devices")
-    launches = [x for g in lists for x in g.launches]
-    with _on(dev):
-        room = sum(part.partials for part, _, _ in launches)
-        partials = torch.empty(max(room, 1), dtype=torch.float64, device=dev)
-        words = torch.empty(4, dtype=torch.float32, device=dev) if out is None else out
-        if out is not None and (_chk(out, name="out") is None or out.numel() != 4 or out.device != dev):
-            raise ValueError("grad_norm: out must have 4 elements on %s" % dev)
-        stream, used, base = _stream(), ctypes.c_int64(), partials.data_ptr()
-        at = 0
-        for part, kind, ptrs in launches:
-            _lib.check(lib.benerf_grad_norm_partial(part.host, part.on_device(), ptrs, kind, base + 8 * at, room - at, ctypes.byref(used), stream),
-                       "grad_norm_partial")
-            at += used.value
-        cs = None
-        if counters:
-            cs = (ctypes.c_void_p * len(counters))(*[_counter(c, dev) for c in counters])
-        _lib.check(lib.benerf_grad_norm_finish(base, at, max_norm, grad_scale, words.data_ptr(), int(out is not None),
-                                               _guard_words(dev, guard_range, status), cs, len(counters), stream), "grad_norm_finish")
+    if dev.index != torch.cuda.current_device():
+        with torch.cuda.device(dev):
+            return grad_norm(lists, max_norm, grad_scale, out, counters, guard_range, status)
+    lib = _lib.load()
+    words = torch.empty(4, dtype=torch.float32, device=dev) if out is None else out
+    at = words.data_ptr() if out is None else _norm_words(out, dev, "out")
+    partials = torch.empty(room, dtype=torch.float64, device=dev)
+    steps = (ctypes.c_void_p * len(counters))(*[_counter(c, dev) for c in counters]) if counters else None
+    guard = (mlp_status(dev) if status is None else status).data_ptr() if guard_range else None
+    stream = _stream()
+    for g in lists:
+        for part, _, _ in g.launches:
+            part.used_on(stream)
+    _lib.check(lib.benerf_grad_norm(rows, len(rows), partials.data_ptr(), room, max_norm, grad_scale, at, out is not None, guard, steps, len(counters), stream),
+               "grad_norm")
     return words
-
-
-def _counter(t, device):
-    if t.numel() != 1 or t.device != device:
-        raise ValueError("a counter on the device is one float32 on %s" % device)
-    return _chk(t, name="counter")
 
 
 def adamw_count(step, norm=None, guard_range=True, status=None):
     """One device step counter (float32, 1 element) goes up by one, unless `norm` or the range guard says that the step is skipped."""
-    with _on(step.device):
-        _lib.check(_lib.load().benerf_adamw_count(_counter(step, step.device), _chk(norm, name="norm"), _guard_words(step.device, guard_range, status),
-                                                  _stream()), "adamw_count")
+    dev = step.device
+    if not step.is_cuda:
+        _chk(step, name="step")
+    with torch.cuda.device(dev):
+        guard = (mlp_status(dev) if status is None else status).data_ptr() if guard_range else None
+        _lib.check(_lib.load().benerf_adamw_count(_counter(step, dev), None if norm is None else _norm_words(norm, dev, "norm"), guard, _stream()), "adamw_count")
 
 
 def adamw_step(plan, grads, lr, step, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.0, grad_scale=1.0, norm=None, seed=0, guard_range=True, status=None):
@@ -938,27 +934,31 @@ def adamw_step(plan, grads, lr, step, betas=(0.9, 0.999), eps=1e-8, weight_decay
     count) - needed in a captured step, whose numbers are frozen.  norm: what grad_norm returned - clips, and skips the step where it says
     so; without a device counter t then counts applied steps.  seed: stochastic rounding of 8-bit moments.  guard_range, status: as in
     `adam_step`."""
-    lib = _lib.load()
-    grads = _as_grads(grads, plan)
-    cfg = _lib.AdamwCfg(beta1=betas[0], beta2=betas[1], eps=eps, weight_decay=weight_decay, grad_scale=grad_scale, seed=int(seed) & 0xFFFFFFFFFFFFFFFF)
     dev = plan.device
-    with _on(dev):
-        if torch.is_tensor(step):
-            cfg.step_dev = _counter(step, dev)
-        else:
-            if torch.cuda.is_current_stream_capturing():
-                raise _lib.BenerfHipError("adamw_step: a captured step needs its counter on the device (step=tensor)")
-            cfg.step = int(step)
-        if torch.is_tensor(lr):
-            cfg.lr_dev = _counter(lr, dev)
-        else:
-            cfg.lr = lr
-        if norm is not None and (norm.numel() != 4 or norm.device != dev):
-            raise ValueError("adamw_step: norm must be the 4 words of grad_norm on %s" % dev)
-        words, guard, stream = _chk(norm, name="norm"), _guard_words(dev, guard_range, status), _stream()
-        launches = grads.launches if grads.parts is plan.parts else _grad_launches(plan.parts, grads.tensors)
-        for part, kind, ptrs in launches:
-            _lib.check(lib.benerf_adamw_step(part.host, part.on_device(), ptrs, kind, ctypes.byref(cfg), words, guard, stream), "adamw_step")
+    if dev.index != torch.cuda.current_device():
+        with torch.cuda.device(dev):
+            return adamw_step(plan, grads, lr, step, betas, eps, weight_decay, grad_scale, norm, seed, guard_range, status)
+    if isinstance(grads, GradList) and grads.parts is plan.parts:
+        launches = grads.launches
+    else:
+        launches = _grad_launches(plan.parts, _as_grads(grads, plan).tensors)
+    lib = _lib.load()
+    t = lr_dev = step_dev = None
+    if torch.is_tensor(step):
+        step_dev = _counter(step, dev)
+    elif torch.cuda.is_current_stream_capturing():
+        raise _lib.BenerfHipError("adamw_step: a captured step needs its counter on the device (step=tensor)")
+    else:
+        t = int(step)
+    if torch.is_tensor(lr):
+        lr_dev, lr = _counter(lr, dev), 0.0
+    cfg = _lib.AdamwCfg(lr, betas[0], betas[1], eps, weight_decay, grad_scale, t or 0, int(seed) & 0xFFFFFFFFFFFFFFFF, lr_dev, step_dev)
+    words = None if norm is None else _norm_words(norm, dev, "norm")
+    guard = (plan.guard if status is None else status.data_ptr()) if guard_range else None
+    stream = _stream()
+    for part, kind, ptrs in launches:
+        part.used_on(stream)
+        _lib.check(lib.benerf_adamw_step(part.host_at, part.dev_at, ptrs.buffer_info()[0], kind, cfg, words, guard, stream), "adamw_step")
     params_changed()
 
 

@@ -23,8 +23,10 @@ update rule (weight_decay, amsgrad, maximize) are refused: the reference never s
 a synchronisation, moments in 32 or 8 bits, float32 master copies of half-precision parameters.
 """
 import itertools
+from operator import is_, itemgetter
 
 import torch
+from torch.optim.optimizer import _global_optimizer_post_hooks, _global_optimizer_pre_hooks
 
 from . import kernels as K
 
@@ -241,12 +243,25 @@ class _Cohort:
 
 
 class _Group:
-    """What a step needs of one parameter group, made once and again when something moved."""
+    """What a step needs of one parameter group, made once and again when something was replaced or moved."""
+    PARTS = itemgetter("exp_avg", "exp_avg_sq", "step")
 
     def __init__(self, params, plan, states, cohorts):
         self.params, self.plan, self.states, self.cohorts = params, plan, states, cohorts
         self.at = [p.data_ptr() for p in params]
-        self.kept = [(st, st["exp_avg"], st["exp_avg_sq"], st["step"]) for st in states]
+        self.look()
+
+    def look(self):
+        self.parts = list(itertools.chain.from_iterable(map(self.PARTS, self.states)))
+
+    def holds(self, params):
+        """Parameters, their addresses and their state are the ones that the plan was made for."""
+        return (len(params) == len(self.params) and all(map(is_, params, self.params)) and [p.data_ptr() for p in params] == self.at and
+                all(map(is_, itertools.chain.from_iterable(map(self.PARTS, self.states)), self.parts)))
+
+
+def _hooks_or_profiler():
+    return bool(_global_optimizer_pre_hooks or _global_optimizer_post_hooks or torch.autograd.profiler._is_profiler_enabled)
 
 
 class FusedAdamW(torch.optim.AdamW):
@@ -264,6 +279,7 @@ class FusedAdamW(torch.optim.AdamW):
       capturable  counters live on the device, a step can be captured (make one step before, outside; learning rates that change need
                   `lr` as a float32 tensor on the device).  With max_norm they live there too.
       guard_range skip the step where the MLP's range guard says so, like FlatAdam.
+    state[p]["step"] is ONE tensor for all parameters of a group that have made the same steps (state_dict gives each its own).
     amsgrad, maximize and differentiable are refused."""
 
     STATE_KEYS = ("exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale", "master")
@@ -275,7 +291,7 @@ class FusedAdamW(torch.optim.AdamW):
         if max_norm is not None and not max_norm > 0:
             raise ValueError("FusedAdamW: max_norm must be positive, got %r" % (max_norm,))
         self._settings = dict(state_bits=state_bits, max_norm=max_norm, master=bool(master), seed=int(seed), guard_range=bool(guard_range))
-        self._plans = {}
+        self._plans, self._states = {}, []
         self.grad_norm = None
         super().__init__(params, lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, capturable=capturable, **kw)
 
@@ -287,8 +303,16 @@ class FusedAdamW(torch.optim.AdamW):
 
     def __setstate__(self, state):
         super().__setstate__(state)
-        self._plans = {}
+        self._plans, self._states = {}, []
         self.grad_norm = None
+
+    def state_dict(self):
+        # every parameter gets a counter of its own: torch's AdamW, loading this, adds to each of them.  On the host, as torch keeps it.
+        out = super().state_dict()
+        on_device = {k for g in out["param_groups"] if g.get("capturable") for k in g["params"]}
+        out["state"] = {k: dict(st, step=st["step"].clone() if k in on_device else st["step"].cpu().clone()) if torch.is_tensor(st.get("step")) else st
+                        for k, st in out["state"].items()}
+        return out
 
     def load_state_dict(self, state_dict):
         super().load_state_dict(state_dict)
@@ -352,6 +376,7 @@ class FusedAdamW(torch.optim.AdamW):
                     x = st.get("master")
                     st["master"] = p.detach().float() if x is None else x.to(device=p.device, dtype=torch.float32).contiguous()
 
+    @torch.no_grad()
     def _make(self, group):
         params = list(group["params"])
         self._adopt(params)
@@ -376,55 +401,72 @@ class FusedAdamW(torch.optim.AdamW):
 
     def _group(self, index, group):
         g = self._plans.get(index)
-        if g is not None and len(g.params) == len(group["params"]):
-            state = self.state
-            for p, q, at, n, (st, m, v, step) in zip(group["params"], g.params, g.at, g.plan.numels, g.kept):
-                if p is not q or p.data_ptr() != at or p.numel() != n or state.get(p) is not st or st["exp_avg"] is not m or st["exp_avg_sq"] is not v or st["step"] is not step:
-                    break
-            else:
-                return g
-        g = self._plans[index] = self._make(group)
+        if g is None or not g.holds(group["params"]):
+            g = self._plans[index] = self._make(group)
+            self._states = list(self.state.values())
         return g
 
+    @staticmethod
+    def _gradients(g):
+        """The group's gradients, contiguous, and whether some are missing."""
+        grads = [p.grad for p in g.params]
+        sizes, index = g.plan.numels, g.plan.device.index
+        if any([x is None for x in grads]):
+            sizes, there = [n for n, x in zip(sizes, grads) if x is not None], [x for x in grads if x is not None]
+        else:
+            there = grads
+        if [x.numel() for x in there] != sizes or any([x.get_device() != index for x in there]):     # p.data was replaced behind its gradient
+            raise RuntimeError("FusedAdamW: a gradient has another size or device than its parameter")
+        if not all([x.is_contiguous() for x in there]):
+            if any([x.layout is not torch.strided for x in there]):
+                raise NotImplementedError("FusedAdamW: sparse gradients")
+            grads = [x if x is None else x.detach().contiguous() for x in grads]
+        return grads, len(there) < len(grads)
+
     # -- the update ----------------------------------------------------------------------------------------------------------
-    @torch.no_grad()
     def step(self, closure=None):
+        # torch wraps step() of every optimiser with its hooks and a profiler range, at 10 us a call: only where there are any
+        if self._optimizer_step_pre_hooks or self._optimizer_step_post_hooks or _hooks_or_profiler():
+            return self._hooked_step(closure)
+        return self._step(closure)
+
+    step.hooked = True
+
+    def _step(self, closure=None):
         loss = None
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        work, norms = [], []
+        if len(self.state) != len(self._states) or not all(map(is_, self.state.values(), self._states)):
+            self._plans = {}                # state[p] was assigned
+        work, norms = [], []                # (group's place, group, plan and counters, cohort, its gradients)
         for index, group in enumerate(self.param_groups):
-            if group.get("amsgrad") or group.get("maximize") or group.get("differentiable"):
+            if group["amsgrad"] or group["maximize"] or group["differentiable"]:
                 raise NotImplementedError("FusedAdamW: amsgrad, maximize and differentiable are not built")
             if not group["params"]:
                 continue
             g = self._group(index, group)
-            grads = [self._gradient(p, n) for p, n in zip(g.params, g.plan.numels)]
-            if all(x is None for x in grads):
-                continue
-            if any(x is None for x in grads):
+            grads, missing = self._gradients(g)
+            if missing:
+                if all(x is None for x in grads):
+                    continue
                 self._split(g, grads)
             whole = K.GradList.of_checked(grads, g.plan)
             norms.append(whole)
             for c in g.cohorts:
-                if grads[c.members[0]] is None:
-                    continue
                 if len(c.members) == len(grads):
-                    part = whole
-                else:
+                    work.append((index, group, g, c, whole))
+                elif grads[c.members[0]] is not None:
                     mine = set(c.members)
-                    part = K.GradList.of_checked([x if k in mine else None for k, x in enumerate(grads)], g.plan)
-                work.append((index, group, g, c, part))
+                    work.append((index, group, g, c, K.GradList.of_checked([x if k in mine else None for k, x in enumerate(grads)], g.plan)))
         if not work:
             return loss
-        guard = self._settings["guard_range"]
-        words = None
+        guard, words = self._settings["guard_range"], None
         on_device = [c.step for _, group, _, c, _ in work if self._counts_on_device(group)]
         if self.max_norm is not None:
             if self.grad_norm is None:
                 self.grad_norm = torch.zeros(4, dtype=torch.float32, device=norms[0].device)
-            words = K.grad_norm(norms, self.max_norm, out=self.grad_norm, counters=on_device[:64], guard_range=guard)
+            words = K.grad_norm(norms[0] if len(norms) == 1 else norms, self.max_norm, out=self.grad_norm, counters=on_device[:64], guard_range=guard)
             on_device = on_device[64:]
         for s in on_device:
             K.adamw_count(s, norm=words, guard_range=guard)
@@ -437,16 +479,7 @@ class FusedAdamW(torch.optim.AdamW):
                 c.step += 1.0
         return loss
 
-    @staticmethod
-    def _gradient(p, n):
-        x = p.grad
-        if x is None:
-            return None
-        if x.layout is not torch.strided:
-            raise NotImplementedError("FusedAdamW: sparse gradients")
-        if x.numel() != n or x.get_device() != p.get_device():      # p.data was replaced by something else behind its gradient
-            raise RuntimeError("FusedAdamW: a gradient has another size or device than its parameter")
-        return x if x.is_contiguous() else x.contiguous()
+    _hooked_step = torch.optim.Optimizer.profile_hook_step(_step)
 
     def _split(self, g, grads):
         """Cohorts in which only some have a gradient this time part: the others' counter stays."""
@@ -457,5 +490,5 @@ class FusedAdamW(torch.optim.AdamW):
                 new = _Cohort(c.step.clone(), have)
                 for k in have:
                     g.states[k]["step"] = new.step
-                    g.kept[k] = g.kept[k][:3] + (new.step,)
                 g.cohorts.append(new)
+        g.look()

@@ -411,7 +411,7 @@ int benerf_adam_step(float* param, const float* grad, float* exp_avg, float* exp
  *   state_bits 32: exp_avg, exp_avg_sq float32 [n], the scale pointers are not read;
  *   state_bits 8:  exp_avg uint8 [n] e4m3 codes of m, exp_avg_sq uint8 [n] e4m3 codes of sqrt(v), *_scale float32 [ceil(n / 128)]: the
  *                  power of two that belongs to 128 consecutive elements (0 moments: any scale with codes 0);
- *   state_bits 0:  a plan for benerf_grad_norm_partial alone, only n is read (param_type: the gradients').
+ *   state_bits 0:  a plan for benerf_grad_norm alone, only n is read (param_type: the gradients').
  *   master: float32 [n], or NULL: the parameter itself is read.  With it, param is written only.
  *   first_block: number of the tensor's first block of 128 in the caller's numbering (8 bits: the generator's counter; give every
  *                tensor its own range).
@@ -435,27 +435,32 @@ typedef struct BenerfAdamwCfg {
     int64_t step;            /* t of this step, from 1; not read with step_dev */
     uint64_t seed;           /* stochastic rounding of 8-bit moments */
     const float* lr_dev;     /* NULL, or one device float that takes the place of lr */
-    const float* step_dev;   /* NULL, or one device float that holds t of this step (benerf_adamw_count / benerf_grad_norm_finish count) */
+    const float* step_dev;   /* NULL, or one device float that holds t of this step (benerf_adamw_count / benerf_grad_norm count) */
 } BenerfAdamwCfg;
 size_t benerf_adamw_plan_bytes(const BenerfAdamwTensor* tensors_host, int n_tensors);       /* 0: bad list */
 int benerf_adamw_plan_fill(const BenerfAdamwTensor* tensors_host, int n_tensors, int param_type, int state_bits, void* plan_host,
                            size_t plan_bytes);
-/* One step over the list.  norm_words: NULL, or what benerf_grad_norm_finish wrote: gradients are multiplied by [1], nothing happens
+/* One step over the list.  norm_words: NULL, or what benerf_grad_norm wrote: gradients are multiplied by [1], nothing happens
  * where [2] is set, and without step_dev t = step - [3].  skip_if_range: as in benerf_adam_step (status words, or NULL). */
 int benerf_adamw_step(const void* plan_host, const void* plan_dev, const void* const* grads_host, int grad_type,
                       const BenerfAdamwCfg* cfg, const float* norm_words, const uint32_t* skip_if_range, benerf_stream_t stream);
 /* *step_dev += 1, unless norm_words or skip_if_range say that the step is skipped: for captured steps without a norm. */
 int benerf_adamw_count(float* step_dev, const float* norm_words, const uint32_t* skip_if_range, benerf_stream_t stream);
-/* Squares of the list's gradients, summed in f64 and in a fixed order, one partial sum per workgroup into partials (device, room for
- * benerf_grad_norm_partials(plan)); *used_host: how many were written.  Several lists (types, groups) write one behind the other. */
-size_t benerf_grad_norm_partials(const void* plan_host);
-int benerf_grad_norm_partial(const void* plan_host, const void* plan_dev, const void* const* grads_host, int grad_type,
-                             double* partials, size_t n_partials, int64_t* used_host, benerf_stream_t stream);
-/* words[4] = { norm = |grad_scale| sqrt(sum), coefficient min(1, max_norm / (norm + 1e-6)), 1 if the step is to be skipped (norm inf or
+/* 2-norm over the gradients of one or several lists (element types, parameter groups).  Squares are summed in f64 and in a fixed order;
+ * partials: device, room for the sum of benerf_grad_norm_partials(plan) over the lists.
+ * words[4] = { norm = |grad_scale| sqrt(sum), coefficient min(1, max_norm / (norm + 1e-6)), 1 if the step is to be skipped (norm inf or
  * NaN, or the status words say so) else 0, number of skipped steps (accumulate: added to what words[3] holds) }.  max_norm > 0, may be
  * infinite.  counters_host: up to 64 step counters (device floats) that go up by one unless the step is skipped. */
-int benerf_grad_norm_finish(const double* partials, int64_t n_partials, double max_norm, double grad_scale, float* words, int accumulate,
-                            const uint32_t* skip_if_range, float* const* counters_host, int n_counters, benerf_stream_t stream);
+typedef struct BenerfGradList {
+    const void* plan_host;
+    const void* plan_dev;
+    const void* const* grads_host;
+    int32_t grad_type;
+} BenerfGradList;
+size_t benerf_grad_norm_partials(const void* plan_host);
+int benerf_grad_norm(const BenerfGradList* lists_host, int n_lists, double* partials, size_t n_partials, double max_norm,
+                     double grad_scale, float* words, int accumulate, const uint32_t* skip_if_range, float* const* counters_host,
+                     int n_counters, benerf_stream_t stream);
 
 #ifdef __cplusplus
 }

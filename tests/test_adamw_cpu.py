@@ -66,18 +66,17 @@ def test_step_and_norm_refusals(lib):
     none = (ctypes.c_void_p * 1)()
     assert step(plan, plan, none, 0, cfg(), None, None, None) == 0           # no gradient at all: nothing to launch
     assert lib.benerf_adamw_count(None, None, None, None) == -1
-    used = ctypes.c_int64(-1)
     assert lib.benerf_grad_norm_partials(plan) == 1 and lib.benerf_grad_norm_partials(None) == 0
-    assert lib.benerf_grad_norm_partial(plan, plan, odd, 0, 0x6000, 1, ctypes.byref(used), None) == -1
-    assert lib.benerf_grad_norm_partial(plan, plan, g, 0, 0x6000, 0, ctypes.byref(used), None) == -2
-    assert lib.benerf_grad_norm_partial(plan, plan, none, 0, 0x6000, 1, ctypes.byref(used), None) == 0 and used.value == 0
-    fin = lib.benerf_grad_norm_finish
-    assert fin(0x6000, 1, 0.0, 1.0, 0x7000, 0, None, None, 0, None) == -1
-    assert fin(0x6000, 1, float("nan"), 1.0, 0x7000, 0, None, None, 0, None) == -1
-    assert fin(0x6000, 1, 1.0, 1.0, None, 0, None, None, 0, None) == -1
-    assert fin(None, 1, 1.0, 1.0, 0x7000, 0, None, None, 0, None) == -1
-    assert fin(0x6000, 1, 1.0, 1.0, 0x7000, 0, None, None, 65, None) == -1
-    assert fin(0x6000, 1, 1.0, 1.0, 0x7000, 0, None, (ctypes.c_void_p * 1)(), 1, None) == -1
+    keep = []
+
+    def norm(g=g, kind=0, host=plan, dev=0x8000, room=1, most=1.0, words=0x7000, partials=0x6000, counters=None, n=0, rows=1):
+        row = (_lib.GradListRow * 1)((None if host is None else ctypes.addressof(host), dev, ctypes.addressof(g) if g is not None else None, kind))
+        keep.append(row)
+        return lib.benerf_grad_norm(row, rows, partials, room, most, 1.0, words, 0, None, counters, n, None)
+    for kw in (dict(g=odd), dict(g=None), dict(kind=3), dict(host=None), dict(dev=None), dict(most=0.0), dict(most=float("nan")), dict(words=None), dict(partials=None),
+               dict(n=65), dict(n=-1), dict(n=1), dict(n=1, counters=(ctypes.c_void_p * 1)()), dict(rows=-1), dict(host=ctypes.create_string_buffer(200))):
+        assert norm(**kw) == -1 and b"grad_norm" in lib.benerf_last_error(), kw
+    assert norm(room=0) == -2
 
 
 def test_python_refusals():
