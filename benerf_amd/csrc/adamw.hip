@@ -110,7 +110,7 @@ __device__ __forceinline__ bool step_scalars(const AdamwArgs& a, Hyper& h, int64
         h.gs = h.gs * a.norm[1];
         skipped = a.norm[3];
     }
-    const uint32_t gated = a.status ? a.status[BENERF_ST_SKIPPED_TOTAL] : 0u;
+    const uint32_t gated = a.status && !a.norm ? a.status[BENERF_ST_SKIPPED_TOTAL] : 0u;      // the norm's count holds them
     if (a.step_dev || a.lr_dev || skipped != 0.f || gated != 0u) {
         t = a.step_dev ? (int64_t)a.step_dev[0] : a.step - (int64_t)skipped - (int64_t)gated;
         if (t < 1) t = 1;

@@ -528,13 +528,29 @@ class TrainStep:
         n_total = 2 * n_net + 24 + 6 + 1 + n_crf
         self.flat_p = torch.zeros(n_total, dtype=torch.float32, device=device)
         self.flat_g = torch.zeros(n_total, dtype=torch.float32, device=device)
-        self.flat_m = torch.zeros(n_total, dtype=torch.float32, device=device)
-        self.flat_v = torch.zeros(n_total, dtype=torch.float32, device=device)
+        # the networks' optimiser (optim.network_settings): the reference's Adam on the flat range, or AdamW on their 48 tensors (K9)
+        self.net_bits, self.net_decay, self.max_grad_norm = optim.network_settings(cfg)
+        self.off_moments = 2 * n_net if self.net_bits == 8 else 0          # 8-bit moments live in buffers of their own
+        self.flat_m = torch.zeros(n_total - self.off_moments, dtype=torch.float32, device=device)
+        self.flat_v = torch.zeros(n_total - self.off_moments, dtype=torch.float32, device=device)
         self.net_c = FlatNet(wc, bc, self.C, self.flat_p, self.flat_g, 0)
         self.net_f = FlatNet(wf, bf, self.C, self.flat_p, self.flat_g, n_net)
         o = 2 * n_net
         kn = graph.evt_knot_pose_se3.params.weight
         tr = graph.transform.params.weight
+        self.net_plan = None
+        if self.net_bits is not None:
+            nets = (self.net_c, self.net_f)
+            params = [x for n_ in nets for x in n_.views_w + n_.views_b]
+            if self.net_bits == 8:
+                self.net_moments = optim.zero_moments(params, 8)
+            else:
+                at = [(x.storage_offset(), x) for x in params]
+                self.net_moments = {name: [flat[k:k + x.numel()].view(x.shape) for k, x in at] for name, flat in (("exp_avg", self.flat_m), ("exp_avg_sq", self.flat_v))}
+            self.net_plan = K.AdamWPlan(params, **self.net_moments)
+            self.net_grads = K.GradList([x for n_ in nets for x in n_.gviews_w + n_.gviews_b], self.net_plan)
+            self.net_steps = torch.zeros((), dtype=torch.float32, device=device)      # applied steps
+            self.net_norm = torch.zeros(4, dtype=torch.float32, device=device)        # K9's words of the last step
         self.knots = self.flat_p[o:o + 24].view(4, 6)
         self.knots.copy_(kn.detach())
         kn.data = self.knots
@@ -596,6 +612,10 @@ class TrainStep:
         assert 0 <= off and off + p.numel() <= self.flat_p.numel(), "parameter is not backed by this TrainStep's flat buffer"
         return off, p.numel()
 
+    def _network_places(self):
+        """{offset in the flat parameter buffer: place in the networks' AdamW plan}, empty with the reference's Adam."""
+        return {} if self.net_plan is None else {x.storage_offset(): k for k, x in enumerate(self.net_plan.params)}
+
     def _trained_optimizers(self, optimizers):
         cfg = self.cfg
         return ((optimizers[0], self._lr(cfg.lrate, cfg.decay_rate)), (optimizers[1], self._lr(cfg.pose_lrate, cfg.decay_rate_pose)),
@@ -607,11 +627,17 @@ class TrainStep:
         count and current learning rates, ready for checkpoint.save (the tone-mapper optimisers too, when they are trained)."""
         # Adam's step count = APPLIED steps (a step the range guard skipped did not touch the moments); synchronises
         applied = self.global_step - int(self.guard.words[_lib.ST_SKIPPED_TOTAL].item())
+        place = self._network_places()
         for opt, lr in self._trained_optimizers(optimizers):
             for group in opt.param_groups:
                 group["lr"] = lr
                 for p in group["params"]:
                     off, n = self._flat_slice(p)
+                    if off in place:        # in the form that the optimiser keeps
+                        held = {name: ts[place[off]].clone() for name, ts in self.net_moments.items()}
+                        opt.state[p] = dict(optim.convert_moments(held, getattr(opt, "state_bits", 32)), step=torch.tensor(float(self.net_steps), device="cpu"))
+                        continue
+                    off -= self.off_moments
                     opt.state[p] = {"step": torch.tensor(float(applied), device="cpu"),
                                     "exp_avg": self.flat_m[off:off + n].view_as(p).clone(),
                                     "exp_avg_sq": self.flat_v[off:off + n].view_as(p).clone()}
@@ -623,6 +649,7 @@ class TrainStep:
         skipped before the checkpoint - goes back into the device's [SKIPPED_TOTAL] word, so that the resumed run's bias
         correction continues exactly where the saved one stopped."""
         applied = None
+        place = self._network_places()
         for opt, _ in self._trained_optimizers(optimizers):
             for group in opt.param_groups:
                 for p in group["params"]:
@@ -630,6 +657,12 @@ class TrainStep:
                     if not st:
                         continue
                     off, n = self._flat_slice(p)
+                    if off in place:
+                        for name, x in optim.convert_moments(st, self.net_bits).items():
+                            self.net_moments[name][place[off]].copy_(x.reshape(self.net_moments[name][place[off]].shape))
+                        self.net_steps.fill_(float(st["step"]))
+                        continue
+                    off -= self.off_moments
                     self.flat_m[off:off + n].copy_(st["exp_avg"].reshape(-1))
                     self.flat_v[off:off + n].copy_(st["exp_avg_sq"].reshape(-1))
                     if "step" in st:
@@ -959,7 +992,8 @@ class TrainStep:
         t = self.global_step + 1
 
         def adam(lo, cnt, lr):
-            K.adam_step(self.flat_p[lo:lo + cnt], self.flat_g[lo:lo + cnt], self.flat_m[lo:lo + cnt], self.flat_v[lo:lo + cnt], lr, t,
+            mo = lo - self.off_moments
+            K.adam_step(self.flat_p[lo:lo + cnt], self.flat_g[lo:lo + cnt], self.flat_m[mo:mo + cnt], self.flat_v[mo:mo + cnt], lr, t,
                         status=st)
         o = self.off_pose
         if cfg.optimize_pose:
@@ -984,7 +1018,16 @@ class TrainStep:
         if loss_sum is not None:
             loss_sum.wait()
         if cfg.optimize_nerf:
-            adam(0, 2 * self.n_net, self._lr(cfg.lrate, cfg.decay_rate))
+            lr_net = self._lr(cfg.lrate, cfg.decay_rate)
+            if self.net_plan is None:
+                adam(0, 2 * self.n_net, lr_net)
+            else:       # the gradients are summed over the ranks by now: every rank finds the same norm and takes the same decision
+                words = None
+                if self.max_grad_norm is None:
+                    K.adamw_count(self.net_steps, status=st)
+                else:
+                    words = K.grad_norm(self.net_grads, self.max_grad_norm, out=self.net_norm, counters=[self.net_steps], status=st)
+                K.adamw_step(self.net_plan, self.net_grads, lr_net, self.net_steps, weight_decay=self.net_decay, norm=words, seed=self.seed, status=st)
         for lo, cnt, lr0, dr, _ in self.crf_groups:
             adam(lo, cnt, self._lr(lr0, dr))
         if self.global_step % self.GUARD_POST_EVERY == 0:

@@ -881,11 +881,11 @@ def _norm_words(t, device, name):
     return _chk(t, name=name)
 
 
-def grad_norm(grads, max_norm=float("inf"), grad_scale=1.0, out=None, counters=(), guard_range=False, status=None):
+def grad_norm(grads, max_norm=float("inf"), grad_scale=1.0, out=None, counters=(), guard_range=True, status=None):
     """2-norm over all gradients of a list (GradList, a list of tensors, or a list of GradLists: one norm over all of them), on the
     device and without synchronising.  Returns float32 [4] = [norm of grad_scale * gradients, coefficient min(1, max_norm / (norm +
     1e-6)), 1 if the step must be skipped (norm not finite, or guard_range and the range guard's words say so), skipped steps so far];
-    hand it to `adamw_step(norm=...)`.  out: such a tensor (zeroed once by the caller) to write, whose count of skipped steps goes on.
+    hand it to `adamw_step(norm=...)`, with the same guard_range and status.  out: such a tensor (zeroed once by the caller) to write, whose count of skipped steps goes on.
     counters: up to 64 float32 1-element step counters on the device that go up by one unless the step is skipped."""
     if not max_norm > 0:
         raise ValueError("grad_norm: max_norm must be positive, got %r" % (max_norm,))

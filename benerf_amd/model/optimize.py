@@ -7,7 +7,7 @@ from .. import engine
 from . import nerf
 from .component import ColorToneMapper, LuminanceToneMapper
 from .component import ControlKnotLieAlgebra, TransformationLieAlgebra
-from ..optim import FlatAdam
+from ..optim import FlatAdam, FusedAdamW, network_settings
 
 
 class Model(nerf.Model):
@@ -36,13 +36,19 @@ class Model(nerf.Model):
 
     def setup_optimizer(self, args):
         """Five Adam optimisers with torch defaults (model/optimize.py:36-55).  They ARE torch.optim.Adam objects (param_groups,
-        state, state_dict format, zero_grad) whose step() is one fused launch over a flat parameter arena: benerf_amd/optim.py."""
+        state, state_dict format, zero_grad) whose step() is one fused launch over a flat parameter arena: benerf_amd/optim.py.
+        Extension: args.benerf_optimizer = "adamw" / "adamw8" gives the networks a FusedAdamW (decoupled decay, clipping, moments in 32
+        or 8 bits: optim.network_settings); the trajectory and the tone-mappers, which no decay should pull anywhere, keep Adam."""
         g = self.graph
         # the reference's parameter order: a checkpoint's optimizer state_dict maps state to parameters BY POSITION (train.py:443-455)
         grad_vars = list(g.nerf.parameters())
         if args.N_importance > 0:
             grad_vars += list(g.nerf_fine.parameters())
-        self.optim_nerf = FlatAdam(params=grad_vars, lr=args.lrate)
+        bits, decay, max_norm = network_settings(args)
+        if bits is None:
+            self.optim_nerf = FlatAdam(params=grad_vars, lr=args.lrate)
+        else:
+            self.optim_nerf = FusedAdamW(grad_vars, lr=args.lrate, weight_decay=decay, state_bits=bits, max_norm=max_norm, seed=int(getattr(args, "benerf_seed", 0)))
         self.optim_pose = FlatAdam(params=list(g.evt_knot_pose_se3.parameters()), lr=args.pose_lrate)
         self.optim_transform = FlatAdam(params=list(g.transform.parameters()), lr=args.transform_lrate)
         self.optim_event_crf = FlatAdam(params=list(g.event_crf.mlp_luminance.parameters()), lr=args.event_crf_lrate)

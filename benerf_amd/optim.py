@@ -126,6 +126,9 @@ class FlatAdam(torch.optim.Adam):
             st = {"step": torch.tensor(0.0, dtype=torch.float32, device="cpu"), "exp_avg": m_view, "exp_avg_sq": v_view}
             self.state[p] = st
         else:
+            if "exp_avg_scale" in st:           # FusedAdamW's 8-bit form
+                st.update(convert_moments(st, 32))
+                del st["exp_avg_scale"], st["exp_avg_sq_scale"]
             for key, view in (("exp_avg", m_view), ("exp_avg_sq", v_view)):
                 cur = st.get(key)
                 if cur is None:
@@ -235,6 +238,48 @@ def decode_moment(code, scale):
     return (code.reshape(-1).to(torch.float32) * scale.repeat_interleave(K.ADAMW_BLOCK)[:code.numel()]).view(code.shape)
 
 
+def zero_moments(params, bits):
+    """Moments of a list of parameters at zero, in flat buffers (a tensor's slot at a multiple of 128 elements): the keyword arguments
+    exp_avg, exp_avg_sq - and with 8 bits exp_avg_scale, exp_avg_sq_scale - of kernels.AdamWPlan."""
+    B, out = K.ADAMW_BLOCK, {}
+    blocks = [-(-p.numel() // B) for p in params]
+    starts = list(itertools.accumulate(blocks, initial=0))
+    for name in ("exp_avg", "exp_avg_sq"):
+        flat = torch.zeros(starts[-1] * B, dtype=torch.uint8 if bits == 8 else torch.float32, device=params[0].device)
+        if bits == 8:
+            flat = flat.view(K.CODE_TYPE)
+            scale = torch.zeros(starts[-1], dtype=torch.float32, device=params[0].device)
+            out[name + "_scale"] = [scale[a:a + b] for a, b in zip(starts, blocks)]
+        out[name] = [flat[a * B:a * B + p.numel()].view(p.shape) for a, p in zip(starts, params)]
+    return out
+
+
+def convert_moments(state, bits):
+    """A parameter's saved moments in the form that `bits` asks for, as a new dict of the tensors zero_moments names."""
+    coded = "exp_avg_scale" in state
+    if coded == (bits == 8):
+        return {k: state[k] for k in ("exp_avg", "exp_avg_sq") + (("exp_avg_scale", "exp_avg_sq_scale") if coded else ())}
+    if coded:
+        return {"exp_avg": decode_moment(state["exp_avg"], state["exp_avg_scale"]), "exp_avg_sq": decode_moment(state["exp_avg_sq"], state["exp_avg_sq_scale"]).square_()}
+    out = {}
+    out["exp_avg"], out["exp_avg_scale"] = encode_moment(state["exp_avg"].to(torch.float32))
+    out["exp_avg_sq"], out["exp_avg_sq_scale"] = encode_moment(state["exp_avg_sq"].to(torch.float32).sqrt())
+    return out
+
+
+def network_settings(args):
+    """(state_bits or None for the reference's Adam, weight decay, max_norm) of the networks' optimiser: args.benerf_optimizer "adam"
+    (default), "adamw" or "adamw8" (moments in 8 bits), args.benerf_weight_decay (0.01), args.benerf_max_grad_norm (None: no clipping)."""
+    kind, most = getattr(args, "benerf_optimizer", "adam"), getattr(args, "benerf_max_grad_norm", None)
+    if kind not in ("adam", "adamw", "adamw8"):
+        raise ValueError("benerf_optimizer must be adam, adamw or adamw8, not %r" % (kind,))
+    if kind == "adam":
+        if most is not None or getattr(args, "benerf_weight_decay", 0):
+            raise ValueError("benerf_max_grad_norm and benerf_weight_decay need benerf_optimizer adamw or adamw8")
+        return None, 0.0, None
+    return 8 if kind == "adamw8" else 32, float(getattr(args, "benerf_weight_decay", 1e-2)), most
+
+
 class _Cohort:
     """Parameters of a group that have made the same steps: one counter (torch's `step`), shared by their state dicts."""
 
@@ -333,42 +378,29 @@ class FusedAdamW(torch.optim.AdamW):
 
     def _adopt(self, params):
         """state[p] of every parameter in the form this optimiser keeps: what fits stays where it is, another form is converted, what
-        is missing starts at zero (flat buffers, a tensor's slot at a multiple of 128 elements)."""
+        is missing starts at zero."""
         bits = self.state_bits
-        kind = K.CODE_TYPE if bits == 8 else torch.float32
-        B = K.ADAMW_BLOCK
-        need = {"exp_avg": [], "exp_avg_sq": []}
+        fresh = []
         for p in params:
             st = self.state[p]
-            if bits == 32 and "exp_avg_scale" in st:
-                st["exp_avg"] = decode_moment(st["exp_avg"], st.pop("exp_avg_scale"))
-                st["exp_avg_sq"] = decode_moment(st["exp_avg_sq"], st.pop("exp_avg_sq_scale")).square_()
-            for name, ts in need.items():
-                x = st.get(name)
-                if x is None:
-                    ts.append(p)
-                elif x.numel() != p.numel():
-                    raise ValueError("FusedAdamW: state %s has %d elements, its parameter %d" % (name, x.numel(), p.numel()))
-                elif bits == 8 and name + "_scale" not in st:
-                    x = x.to(device=p.device, dtype=torch.float32)
-                    st[name], st[name + "_scale"] = encode_moment(x.sqrt() if name == "exp_avg_sq" else x)
-                else:
-                    st[name] = x.to(device=p.device, dtype=kind).contiguous()
-                    if bits == 8:
-                        st[name + "_scale"] = st[name + "_scale"].to(device=p.device, dtype=torch.float32).contiguous()
-        for name, ts in need.items():
-            blocks = [-(-p.numel() // B) for p in ts]
-            if not ts:
+            if "exp_avg" not in st or "exp_avg_sq" not in st:
+                fresh.append(p)
                 continue
-            flat = torch.zeros(sum(blocks) * B, dtype=torch.uint8 if bits == 8 else torch.float32, device=ts[0].device)
-            flat = flat.view(kind)
-            scale = torch.zeros(sum(blocks), dtype=torch.float32, device=ts[0].device) if bits == 8 else None
-            at = 0
-            for p, b in zip(ts, blocks):
-                self.state[p][name] = flat[at * B:at * B + p.numel()].view(p.shape)
-                if bits == 8:
-                    self.state[p][name + "_scale"] = scale[at:at + b]
-                at += b
+            for x in (st["exp_avg"], st["exp_avg_sq"]):
+                if x.numel() != p.numel():
+                    raise ValueError("FusedAdamW: a moment has %d elements, its parameter %d" % (x.numel(), p.numel()))
+            if bits == 32:
+                form = convert_moments(st, 32)
+                st.pop("exp_avg_scale", None), st.pop("exp_avg_sq_scale", None)
+            else:
+                form = convert_moments(st, 8)
+            for name, x in form.items():
+                kind = K.CODE_TYPE if bits == 8 and not name.endswith("_scale") else torch.float32
+                st[name] = x.to(device=p.device, dtype=kind).contiguous()
+        if fresh:
+            for name, ts in zero_moments(fresh, bits).items():
+                for p, x in zip(fresh, ts):
+                    self.state[p][name] = x
         if self._settings["master"]:
             for p in params:
                 st = self.state[p]

@@ -441,7 +441,8 @@ size_t benerf_adamw_plan_bytes(const BenerfAdamwTensor* tensors_host, int n_tens
 int benerf_adamw_plan_fill(const BenerfAdamwTensor* tensors_host, int n_tensors, int param_type, int state_bits, void* plan_host,
                            size_t plan_bytes);
 /* One step over the list.  norm_words: NULL, or what benerf_grad_norm wrote: gradients are multiplied by [1], nothing happens
- * where [2] is set, and without step_dev t = step - [3].  skip_if_range: as in benerf_adam_step (status words, or NULL). */
+ * where [2] is set, and without step_dev t = step - [3] (hand benerf_grad_norm the same skip_if_range, then that counts all skipped
+ * steps).  skip_if_range: as in benerf_adam_step (status words, or NULL). */
 int benerf_adamw_step(const void* plan_host, const void* plan_dev, const void* const* grads_host, int grad_type,
                       const BenerfAdamwCfg* cfg, const float* norm_words, const uint32_t* skip_if_range, benerf_stream_t stream);
 /* *step_dev += 1, unless norm_words or skip_if_range say that the step is skipped: for captured steps without a norm. */

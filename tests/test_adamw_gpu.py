@@ -274,6 +274,19 @@ def test_guard_words_skip_and_count(K):
     L.check(before, t=4)
     K.adamw_count(count, status=st)
     assert count.item() == 1.0
+    # with a norm its count is the only one: steps that the guard skipped are in it once
+    words = torch.zeros(4, device="cuda")
+    L = List(K, [500], t=4)
+    for it in range(6):
+        st[_lib.ST_SKIP] = int(it in (1, 2))
+        st[_lib.ST_SKIPPED_TOTAL] += int(it in (1, 2))
+        before = L.snapshot()
+        K.grad_norm(L.g, float("inf"), out=words, status=st)
+        K.adamw_step(L.plan, L.g, step=it + 1, norm=words, status=st, **HYPER)
+        if it in (1, 2):
+            assert all(np.array_equal(a, b) for a, b in zip(before[0], L.state(0)))
+        else:
+            L.check(before, t=it + 1 - int(it > 1) - int(it > 2))
 
 
 @pytest.mark.parametrize("bits", [32, 8])
