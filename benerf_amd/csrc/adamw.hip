@@ -23,7 +23,7 @@ namespace {
 constexpr int THREADS = 128;
 constexpr int BLOCK = BENERF_ADAMW_BLOCK;
 constexpr int CHUNK = THREADS * 4;           // elements a workgroup of the step takes: four a thread
-constexpr int64_t PAST_BYTES = 256ll << 20;  // what the memory-side cache holds
+constexpr int64_t PAST_BYTES = 320ll << 20;  // see Shape
 constexpr uint32_t PLAN_MAGIC = 0x41445731u;
 static_assert(BLOCK == 128, "a block is half a wavefront of four elements a lane");
 
@@ -86,9 +86,12 @@ struct AdamwArgs {
     int64_t step;
     uint64_t seed;
 };
+static_assert(sizeof(AdamwArgs) + sizeof(Ptrs<PTRS_LARGE>) <= 4096, "a launch's arguments");
 
 __device__ __forceinline__ bool guard_says_skip(const uint32_t* st) {
-    return st && (st[BENERF_ST_SKIP] != 0u || st[BENERF_ST_ACT] >= 0x477fe000u || st[BENERF_ST_GRAD] >= 0x477fe000u);
+    if (!st) return false;
+    const uint32_t skip = st[BENERF_ST_SKIP], act = st[BENERF_ST_ACT], grad = st[BENERF_ST_GRAD];
+    return skip != 0u || act >= 0x477fe000u || grad >= 0x477fe000u;
 }
 
 __host__ __device__ inline double int_power(double b, int64_t t) {
@@ -98,26 +101,38 @@ __host__ __device__ inline double int_power(double b, int64_t t) {
     return r;
 }
 
+// 1 / x and 1 / sqrt(x) in f64 from the instructions' estimates (2^-14 at worst) and two steps of Newton's method: as good as f32 needs it
+// several times over, at a tenth of a division's latency
+__device__ __forceinline__ double reciprocal(double x) {
+    double r = __builtin_amdgcn_rcp(x);
+    r = __builtin_fma(__builtin_fma(-x, r, 1.0), r, r);
+    return __builtin_fma(__builtin_fma(-x, r, 1.0), r, r);
+}
+__device__ __forceinline__ double reciprocal_root(double x) {
+    double r = __builtin_amdgcn_rsq(x);
+    r = __builtin_fma(__builtin_fma(-x * r, r, 1.0), 0.5 * r, r);
+    return __builtin_fma(__builtin_fma(-x * r, r, 1.0), 0.5 * r, r);
+}
+
 // Scalars of this step; false: skipped.  What the host could not know (a counter or a learning rate on the device, steps skipped so
 // far) is worked out again here, in f64: 40 multiplications for t < 2^20, once per wave, uniform.
 __device__ __forceinline__ bool step_scalars(const AdamwArgs& a, Hyper& h, int64_t& t) {
-    if (guard_says_skip(a.status)) return false;
-    h = a.h;
-    t = a.step;
-    float skipped = 0.f;
-    if (a.norm) {
-        if (a.norm[2] != 0.f) return false;
-        h.gs = h.gs * a.norm[1];
-        skipped = a.norm[3];
-    }
+    // all words that may matter are read before any of them is looked at
+    const bool guard = guard_says_skip(a.status);
     const uint32_t gated = a.status && !a.norm ? a.status[BENERF_ST_SKIPPED_TOTAL] : 0u;      // the norm's count holds them
+    const float coef = a.norm ? a.norm[1] : 1.f, verdict = a.norm ? a.norm[2] : 0.f, skipped = a.norm ? a.norm[3] : 0.f;
+    const float counted = a.step_dev ? a.step_dev[0] : 0.f, rate = a.lr_dev ? a.lr_dev[0] : 0.f;
+    if (guard || verdict != 0.f) return false;
+    h = a.h;
+    h.gs = h.gs * coef;
+    t = a.step;
     if (a.step_dev || a.lr_dev || skipped != 0.f || gated != 0u) {
-        t = a.step_dev ? (int64_t)a.step_dev[0] : a.step - (int64_t)skipped - (int64_t)gated;
+        t = a.step_dev ? (int64_t)counted : a.step - (int64_t)skipped - (int64_t)gated;
         if (t < 1) t = 1;
-        const double lr = a.lr_dev ? (double)a.lr_dev[0] : a.lr;
+        const double lr = a.lr_dev ? (double)rate : a.lr;
         h.decay = (float)(1.0 - lr * a.decay_rate);
-        h.step_size = (float)(lr / (1.0 - int_power(a.beta1, t)));
-        h.inv_bc2 = (float)(1.0 / sqrt(1.0 - int_power(a.beta2, t)));
+        h.step_size = (float)(lr * reciprocal(1.0 - int_power(a.beta1, t)));
+        h.inv_bc2 = (float)reciprocal_root(1.0 - int_power(a.beta2, t));
     }
     return true;
 }
@@ -464,6 +479,7 @@ struct Counters {
 __global__ __launch_bounds__(NORM_THREADS) void grad_norm_finish_kernel(const double* partials, int n, double max_norm, double grad_scale, float* words, int accumulate,
                                                                    const uint32_t* status, Counters counters) {
     double acc = 0.0;
+#pragma unroll 4
     for (int k = threadIdx.x; k < n; k += NORM_THREADS) acc += partials[k];
     const double s = group_sum(acc);
     if (threadIdx.x != 0) return;
@@ -479,8 +495,9 @@ __global__ __launch_bounds__(NORM_THREADS) void grad_norm_finish_kernel(const do
 }
 
 // ---- host ------------------------------------------------------------------------------------------------------------------
-// of a list: SHORT, or MANY where a launch of the small kind cannot carry its addresses; PAST: more than the memory-side cache holds from
-// one step to the next, so it is read and written past the caches
+// of a list: SHORT, or MANY where a launch of the small kind cannot carry its addresses; PAST: more than the memory-side cache (256 MB) keeps
+// from one step to the next, so it is read and written past the caches.  32-bit step over parameters, gradients and moments of 192 MB: 52 us
+// through them, 57 past them; 256 MB 70 / 75; 320 MB 93 / 94; 384 MB 131 / 111; 2 GB 739 / 600 (6.3 TB/s); 8 bits alike.
 enum Shape { SHORT, MANY, PAST };
 int type_bytes(int type) { return type == BENERF_F32 ? 4 : 2; }
 int per_launch(int shape) { return shape == SHORT ? PTRS_SMALL : PTRS_LARGE; }

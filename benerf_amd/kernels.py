@@ -722,12 +722,12 @@ class _Part:
         size = lib.benerf_adamw_plan_bytes(table, n)
         if size == 0:
             raise ValueError("a tensor of the list is too large")
-        self.host = ctypes.create_string_buffer(size)
-        _lib.check(lib.benerf_adamw_plan_fill(table, n, param_type, state_bits, self.host, size), "adamw_plan_fill")
-        self.state_bits = state_bits
+        whole = ctypes.create_string_buffer(size)
+        _lib.check(lib.benerf_adamw_plan_fill(table, n, param_type, state_bits, whole, size), "adamw_plan_fill")
+        self.host = ctypes.create_string_buffer(bytes(memoryview(whole)[:64 + 16 * n]))      # what calls read of it
         with torch.cuda.device(device):
             # a blocking copy: the plan is there before anything is queued on any stream
-            self.dev = torch.frombuffer(bytearray(self.host.raw), dtype=torch.uint8).to(device)
+            self.dev = torch.frombuffer(whole, dtype=torch.uint8).to(device)
             self.stream = _stream()
         self.host_at, self.dev_at = ctypes.addressof(self.host), self.dev.data_ptr()
         self.partials = int(lib.benerf_grad_norm_partials(self.host))
@@ -782,7 +782,7 @@ def _grad_launches(parts, tensors):
         kinds = [None if t is None else t.dtype for t in mine]
         if kinds.count(kinds[0]) == len(kinds):
             if kinds[0] is not None:
-                out.append((part, _ELEMENT_TYPES[kinds[0]], array.array("Q", [t.data_ptr() for t in mine])))
+                out.append((part, _ELEMENT_TYPES[kinds[0]], array.array("Q", list(map(torch.Tensor.data_ptr, mine)))))
         else:
             for kind in {k: None for k in kinds if k is not None}:
                 out.append((part, _ELEMENT_TYPES[kind], array.array("Q", [t.data_ptr() if k is kind else 0 for t, k in zip(mine, kinds)])))

@@ -287,13 +287,17 @@ class _Cohort:
         self.step, self.members = step, members
 
 
+# checks of whole lists run through map(): a fifth off what a comprehension of method calls costs
+_address, _numel, _device, _contiguous = torch.Tensor.data_ptr, torch.Tensor.numel, torch.Tensor.get_device, torch.Tensor.is_contiguous
+
+
 class _Group:
     """What a step needs of one parameter group, made once and again when something was replaced or moved."""
     PARTS = itemgetter("exp_avg", "exp_avg_sq", "step")
 
-    def __init__(self, params, plan, states, cohorts):
-        self.params, self.plan, self.states, self.cohorts = params, plan, states, cohorts
-        self.at = [p.data_ptr() for p in params]
+    def __init__(self, params, plan, states, cohorts, on_device):
+        self.params, self.plan, self.states, self.cohorts, self.on_device = params, plan, states, cohorts, on_device
+        self.at = list(map(_address, params))
         self.look()
 
     def look(self):
@@ -301,7 +305,7 @@ class _Group:
 
     def holds(self, params):
         """Parameters, their addresses and their state are the ones that the plan was made for."""
-        return (len(params) == len(self.params) and all(map(is_, params, self.params)) and [p.data_ptr() for p in params] == self.at and
+        return (len(params) == len(self.params) and all(map(is_, params, self.params)) and list(map(_address, params)) == self.at and
                 all(map(is_, itertools.chain.from_iterable(map(self.PARTS, self.states)), self.parts)))
 
 
@@ -321,6 +325,7 @@ class FusedAdamW(torch.optim.AdamW):
       max_norm    None, or the global 2-norm over ALL groups to which gradients are clipped in the same step; a norm that is not finite
                   skips the step on the device.  After step(), grad_norm holds [norm, coefficient, skipped?, steps skipped so far].
       master      float32 copies (state["master"]) of half-precision parameters: read and updated instead of them, rounded into them.
+                  They are made from the parameters at the first step: weights that are loaded later need theirs dropped.
       capturable  counters live on the device, a step can be captured (make one step before, outside; learning rates that change need
                   `lr` as a float32 tensor on the device).  With max_norm they live there too.
       guard_range skip the step where the MLP's range guard says so, like FlatAdam.
@@ -401,15 +406,19 @@ class FusedAdamW(torch.optim.AdamW):
             for name, ts in zero_moments(fresh, bits).items():
                 for p, x in zip(fresh, ts):
                     self.state[p][name] = x
-        if self._settings["master"]:
-            for p in params:
-                st = self.state[p]
+        for p in params:
+            st = self.state[p]
+            if not self._settings["master"]:
+                st.pop("master", None)
+            else:
                 if p.dtype != torch.float32:
                     x = st.get("master")
                     st["master"] = p.detach().float() if x is None else x.to(device=p.device, dtype=torch.float32).contiguous()
 
     @torch.no_grad()
     def _make(self, group):
+        if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("FusedAdamW: make one step outside before a step is captured")
         params = list(group["params"])
         self._adopt(params)
         states = [self.state[p] for p in params]
@@ -419,7 +428,10 @@ class FusedAdamW(torch.optim.AdamW):
         if self._settings["master"] and any(p.dtype != torch.float32 for p in params):
             scales["master"] = [st.get("master") if p.dtype != torch.float32 else None for p, st in zip(params, states)]
         plan = K.AdamWPlan([p.data for p in params], [st["exp_avg"] for st in states], [st["exp_avg_sq"] for st in states], **scales)
-        device = params[0].device if self._counts_on_device(group) else torch.device("cpu")
+        on_device = self._counts_on_device(group)
+        device = plan.device if on_device else torch.device("cpu")
+        if self.max_norm is not None and (self.grad_norm is None or self.grad_norm.device != plan.device):
+            self.grad_norm = torch.zeros(4, dtype=torch.float32, device=plan.device)
         by_value = {}
         for k, st in enumerate(states):
             by_value.setdefault(float(st.get("step", 0.0)), []).append(k)
@@ -429,11 +441,11 @@ class FusedAdamW(torch.optim.AdamW):
             for k in members:
                 states[k]["step"] = c.step
             cohorts.append(c)
-        return _Group(params, plan, states, cohorts)
+        return _Group(params, plan, states, cohorts, on_device)
 
     def _group(self, index, group):
         g = self._plans.get(index)
-        if g is None or not g.holds(group["params"]):
+        if g is None or g.on_device != self._counts_on_device(group) or not g.holds(group["params"]):
             g = self._plans[index] = self._make(group)
             self._states = list(self.state.values())
         return g
@@ -441,16 +453,14 @@ class FusedAdamW(torch.optim.AdamW):
     @staticmethod
     def _gradients(g):
         """The group's gradients, contiguous, and whether some are missing."""
-        grads = [p.grad for p in g.params]
-        sizes, index = g.plan.numels, g.plan.device.index
-        if any([x is None for x in grads]):
+        grads, sizes = [p.grad for p in g.params], g.plan.numels
+        there = grads
+        if any(map(is_, grads, itertools.repeat(None))):
             sizes, there = [n for n, x in zip(sizes, grads) if x is not None], [x for x in grads if x is not None]
-        else:
-            there = grads
-        if [x.numel() for x in there] != sizes or any([x.get_device() != index for x in there]):     # p.data was replaced behind its gradient
+        if list(map(_numel, there)) != sizes or not set(map(_device, there)) <= {g.plan.device.index}:     # p.data was replaced behind its gradient
             raise RuntimeError("FusedAdamW: a gradient has another size or device than its parameter")
-        if not all([x.is_contiguous() for x in there]):
-            if any([x.layout is not torch.strided for x in there]):
+        if not all(map(_contiguous, there)):
+            if any(x.layout is not torch.strided for x in there):
                 raise NotImplementedError("FusedAdamW: sparse gradients")
             grads = [x if x is None else x.detach().contiguous() for x in grads]
         return grads, len(there) < len(grads)
@@ -494,18 +504,18 @@ class FusedAdamW(torch.optim.AdamW):
         if not work:
             return loss
         guard, words = self._settings["guard_range"], None
-        on_device = [c.step for _, group, _, c, _ in work if self._counts_on_device(group)]
+        on_device = [c.step for _, _, g, c, _ in work if g.on_device]
         if self.max_norm is not None:
-            if self.grad_norm is None:
-                self.grad_norm = torch.zeros(4, dtype=torch.float32, device=norms[0].device)
             words = K.grad_norm(norms[0] if len(norms) == 1 else norms, self.max_norm, out=self.grad_norm, counters=on_device[:64], guard_range=guard)
             on_device = on_device[64:]
         for s in on_device:
             K.adamw_count(s, norm=words, guard_range=guard)
         for index, group, g, c, part in work:
-            host = not self._counts_on_device(group)
+            host, lr = not g.on_device, group["lr"]
             t = int(c.step.item()) + 1 if host else c.step
-            K.adamw_step(g.plan, part, group["lr"], t, group["betas"], group["eps"], group["weight_decay"], norm=words,
+            if torch.is_tensor(lr) and not lr.is_cuda:
+                lr = float(lr)
+            K.adamw_step(g.plan, part, lr, t, group["betas"], group["eps"], group["weight_decay"], norm=words,
                          seed=self._settings["seed"] + index * 0x9E3779B97F4A7C15, guard_range=guard)
             if host:
                 c.step += 1.0
@@ -518,6 +528,8 @@ class FusedAdamW(torch.optim.AdamW):
         for c in list(g.cohorts):
             have = [k for k in c.members if grads[k] is not None]
             if have and len(have) < len(c.members):
+                if g.on_device and torch.cuda.is_current_stream_capturing():
+                    raise RuntimeError("FusedAdamW: make one step with the same gradients missing outside before it is captured")
                 c.members = [k for k in c.members if grads[k] is None]
                 new = _Cohort(c.step.clone(), have)
                 for k in have:

@@ -405,12 +405,14 @@ int benerf_adam_step(float* param, const float* grad, float* exp_avg, float* exp
  * same list with a clip coefficient and a verdict that AdamW takes on the device.  Formulas: csrc/adamw.hip.
  *
  * A PLAN describes the list: benerf_adamw_plan_fill writes it into host memory of benerf_adamw_plan_bytes(...) bytes, the caller
- * copies these bytes to the device once and hands both copies to every call.  Gradients are not part of it: every call takes a HOST
+ * copies these bytes to the device once and hands both copies to every call (of the host's copy, the first 64 + 16 n_tensors bytes
+ * are read from then on).  Gradients are not part of it: every call takes a HOST
  * array of n_tensors device pointers (NULL: no gradient this time, the tensor and its moments are left alone), which travel in the
  * launch - a captured launch keeps the addresses it was captured with.  The tensors of a plan must not overlap.
  *   state_bits 32: exp_avg, exp_avg_sq float32 [n], the scale pointers are not read;
  *   state_bits 8:  exp_avg uint8 [n] e4m3 codes of m, exp_avg_sq uint8 [n] e4m3 codes of sqrt(v), *_scale float32 [ceil(n / 128)]: the
- *                  power of two that belongs to 128 consecutive elements (0 moments: any scale with codes 0);
+ *                  power of two that belongs to 128 consecutive elements (0 moments: any scale with codes 0).  inf and NaN in a moment
+ *                  become NaN, of their element alone;
  *   state_bits 0:  a plan for benerf_grad_norm alone, only n is read (param_type: the gradients').
  *   master: float32 [n], or NULL: the parameter itself is read.  With it, param is written only.
  *   first_block: number of the tensor's first block of 128 in the caller's numbering (8 bits: the generator's counter; give every

@@ -310,6 +310,25 @@ def test_non_finite_values_stay_with_themselves(K, bits):
 
 
 @pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("eps", [1e-8, 1e-15])
+def test_values_at_the_ends_of_the_range(K, bits, eps):
+    """Gradients whose squares are denormal or vanish, next to ordinary ones and alone in their block; large ones below the square's end."""
+    L = List(K, [640], bits=bits, seed=13, t=1, zero=True)
+    g = L.g[0]
+    g[0:128] *= 0
+    g[5] = 3e-20                       # alone: its square is denormal
+    g[128:256] = torch.logspace(-25, -17, 128, device="cuda")
+    g[256:384] = torch.logspace(-20, 0, 128, device="cuda")
+    g[384:512] = torch.logspace(10, 18, 128, device="cuda")
+    hyper = dict(HYPER, eps=eps)
+    for t in (1, 2, 3):
+        before = L.snapshot()
+        K.adamw_step(L.plan, L.g, step=t, seed=L.seed, **hyper)
+        L.check(before, t=t, hyper=hyper)
+    assert bool(L.p[0].isfinite().all())
+
+
+@pytest.mark.parametrize("bits", [32, 8])
 def test_counter_and_rate_on_the_device(K, bits):
     L = List(K, [1000, 7], bits=bits, seed=21, t=1)
     step, lr = torch.zeros((), device="cuda"), torch.tensor([HYPER["lr"]], device="cuda")

@@ -310,6 +310,51 @@ def test_captured_optimiser_step(optim, bits, clip):
     assert error and "counter" in error and float(c.state[c.param_groups[0]["params"][0]]["step"]) == 1.0
 
 
+@pytest.mark.parametrize("bits", [32, 8])
+def test_what_a_capture_may_not_begin_with(optim, bits):
+    """A first step, or the first one that misses a gradient, inside a capture: refused, and nothing of the optimiser is left half-made."""
+    ps = _params([(40,), (9,)])
+    o = optim.FusedAdamW(ps, lr=1e-3, state_bits=bits, max_norm=1.0, capturable=True)
+
+    def refused(absent):
+        errors = []
+        for k, p in enumerate(ps):
+            p.grad = None if k in absent else torch.ones_like(p)
+        torch.cuda.synchronize()
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            torch.zeros(1, device="cuda")
+            try:
+                o.step()
+            except RuntimeError as e:
+                errors.append(str(e))
+        return errors
+    before = [p.detach().clone() for p in ps]
+    assert "outside" in refused(())[0] and not any(o.state.values()) and o.grad_norm is None
+    o.step()
+    assert "missing" in refused((1,))[0]
+    assert float(o.state[ps[0]]["step"]) == 1.0 and float(o.state[ps[1]]["step"]) == 1.0
+    for p in ps:
+        p.grad = torch.ones_like(p)
+    o.step()
+    assert all(float(o.state[p]["step"]) == 2.0 for p in ps) and not torch.equal(before[0], ps[0])
+
+
+def test_rates_as_tensors_and_settings_that_change(optim):
+    ps = _params([(50,)])
+    ts = _twins(ps)
+    lr = torch.tensor(1e-2)
+    o, ref = optim.FusedAdamW(ps, lr=lr), torch.optim.AdamW(ts, lr=1e-2)
+    for it in range(4):
+        if it == 2:
+            o.param_groups[0]["capturable"] = True          # counters move to the device, with their values
+            o.param_groups[0]["lr"] = torch.tensor(1e-2, device="cuda")
+        _grads(ps, ts, it)
+        o.step()
+        ref.step()
+    _close(ps, ts, 4, 1e-2, extra=4 * 1e-2 * 2.0 ** -24)
+    assert o.state[ps[0]]["step"].is_cuda and float(o.state[ps[0]]["step"]) == 4.0
+
+
 def test_eight_bits_train_like_thirty_two(optim):
     """The expectation of the stored moments is the moment: over many steps with gradients of constant size the mean of sqrt(v) follows
     its 32-bit value, where rounding to nearest would have stood still at the first step's."""
