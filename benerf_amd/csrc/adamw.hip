@@ -375,13 +375,13 @@ struct Four8 {
 // One workgroup per chunk, four elements a thread.
 template <class PT, class GT, int BITS, bool MASTER, int N, bool PAST>
 __global__ __launch_bounds__(THREADS) void adamw_kernel(AdamwArgs a, Ptrs<N> grads) {
-    const Chunk c = a.chunks[blockIdx.x];
-    const char* gp = static_cast<const char*>(grads.p[c.tensor - a.tensor0]);
-    if (!gp) return;
-    gp += (int64_t)c.index * CHUNK * GT::BYTES;
     Hyper h;
     int64_t t;
-    if (!step_scalars(a, h, t)) return;
+    const bool go = step_scalars(a, h, t);
+    const Chunk c = a.chunks[blockIdx.x];
+    const char* gp = static_cast<const char*>(grads.p[c.tensor - a.tensor0]);
+    if (!gp || !go) return;
+    gp += (int64_t)c.index * CHUNK * GT::BYTES;
     const int i = threadIdx.x * 4;
     typename std::conditional<BITS == 8, Four8<PT, GT, MASTER, PAST>, Four32<PT, GT, MASTER, PAST>>::type f;
     auto chunk = [&](int here) {              // elements there from i on
