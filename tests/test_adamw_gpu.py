@@ -184,8 +184,8 @@ def test_long_lists(K, bits, count):
 
 
 @pytest.mark.parametrize("bits", [32, 8])
-def test_chunks_of_4096(K, bits):
-    """Enough elements for the longer chunks; the last one partial; a large tensor next to small ones."""
+def test_a_large_tensor_next_to_small_ones(K, bits):
+    """Thousands of chunks, so that runs of 64 go to one XCD each; the last one partial."""
     L = List(K, [3, 2200001, 129, 4096, 100003], bits=bits, seed=5)
     before = L.snapshot()
     K.adamw_step(L.plan, L.g, step=L.t, seed=L.seed, **HYPER)
@@ -204,6 +204,25 @@ def test_norm_against_64_bits(K, kind):
             # sums in 64 bits, one rounding to 32: 2^-24, doubled for the root's own
             assert abs(words[0] - norm) <= 2 * O.HALF * norm and abs(words[1] - coef) <= 2 * O.HALF * coef and words[2:] == [0.0, 0.0]
         buf.check()
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("sizes", [[512 * 32], [512 * 32 + 1], [511] * 32, [511] * 33, [1] * 64, [513] * 16, [512 * 31, 1, 1]])
+def test_norm_of_short_lists(K, sizes, kind):
+    """Around the 32 chunks of 512 that one workgroup takes: all gradients, without the last, the first or those between, counted on the device."""
+    gen = torch.Generator().manual_seed(len(sizes))
+    buf = Buffers()
+    g = [buf.put((torch.randn(n, generator=gen) * 0.3).to(TYPES[kind]), shift=1) for n in sizes]
+    words, steps = torch.zeros(4, device="cuda"), [torch.zeros(1, device="cuda") for _ in range(64)]
+    absent = ([], [len(g) - 1], [0], range(1, len(g) - 1))
+    for it, none in enumerate(absent):
+        here = [None if k in none and len(g) > 1 else x for k, x in enumerate(g)]
+        K.grad_norm(here, 0.5, -2.0, out=words, counters=steps)
+        norm, coef = O.clip_words([_f64(x) for x in here if x is not None], 0.5, -2.0)
+        got = words.tolist()
+        assert abs(got[0] - norm) <= 2 * O.HALF * norm and abs(got[1] - coef) <= 2 * O.HALF * coef and got[2:] == [0.0, 0.0]
+        assert all(float(s) == it + 1 for s in steps)
+    buf.check()
 
 
 def test_norm_range_and_verdict(K):
