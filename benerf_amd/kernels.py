@@ -711,11 +711,16 @@ def _list_tensor(t, name, device, dtypes, numel=None):
     return t.detach()
 
 
+_captured = {}                      # plans' tables that captured launches read at every replay: never freed
+
+
 class _Part:
     """The tensors of one element type in a list, and their plan: the host copy and the one on the device."""
 
     def __init__(self, index, rows, param_type, state_bits, device):
         lib = _lib.load()
+        if torch.cuda.is_current_stream_capturing():
+            raise _lib.BenerfHipError("a list of tensors is laid out outside a captured region: make its AdamWPlan or GradList before")
         n = len(rows)
         self.index, self.count = index, n              # places in the list
         table = (_lib.AdamwTensor * n)(*rows)
@@ -731,10 +736,13 @@ class _Part:
             self.stream = _stream()
         self.host_at, self.dev_at = ctypes.addressof(self.host), self.dev.data_ptr()
         self.partials = int(lib.benerf_grad_norm_partials(self.host))
+        self.guard = mlp_status(device).data_ptr()     # the guard's words exist (and are zero) before a launch is captured
 
     def used_on(self, stream):
-        """A launch on `stream` reads the device copy: it must outlive it."""
-        if stream != self.stream:
+        """A launch on `stream` reads the device copy: it must outlive it, and a captured launch all its replays."""
+        if torch.cuda.is_current_stream_capturing():
+            _captured[self.dev_at] = self.dev
+        elif stream != self.stream:
             self.dev.record_stream(torch.cuda.current_stream(self.dev.device))
 
 
@@ -804,15 +812,14 @@ class AdamWPlan:
     ceil(n / 128) elements each (moments in 8 bits; exp_avg_sq then holds the codes of the ROOT of the second moment).  master: None, or
     float32 copies of the parameters that are bfloat16 / float16 (None at the float32 ones): the step reads and updates those and rounds
     them into the parameters.  All tensors are updated where they are; the plan keeps them alive and must be made again when a parameter
-    moves.  Making one copies a table to the device and waits for it: not inside a captured region."""
+    moves.  Making one copies a table to the device and waits for it: not inside a captured region.  Calls for one plan are ordered by
+    the caller, like any writes to its tensors: two streams must not step it at once."""
 
     def __init__(self, params, exp_avg, exp_avg_sq, exp_avg_scale=None, exp_avg_sq_scale=None, master=None):
         params = list(params)
         n = len(params)
         if n == 0:
             raise ValueError("AdamWPlan: empty list")
-        if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
-            raise _lib.BenerfHipError("AdamWPlan: make the plan before the capture")
         self.device = params[0].device if torch.is_tensor(params[0]) else None
         self.params = [_list_tensor(p, "parameter %d" % k, self.device, tuple(_ELEMENT_TYPES)) for k, p in enumerate(params)]
         self.numels = [p.numel() for p in self.params]
@@ -846,7 +853,6 @@ class AdamWPlan:
                     self.master.append(None)
                 else:
                     self.master.append(_list_tensor(t, "master %d" % k, self.device, (torch.float32,), self.numels[k]))
-        self.guard = mlp_status(self.device).data_ptr()       # the guard's words exist (and are zero) before a step can be captured
         _no_overlap([self.params, self.exp_avg, self.exp_avg_sq, self.exp_avg_scale, self.exp_avg_sq_scale, self.master])
         at = lambda l, k: None if l is None or l[k] is None else l[k].data_ptr()       # noqa: E731
         rows, block = {}, 0
@@ -881,6 +887,12 @@ def _norm_words(t, device, name):
     return _chk(t, name=name)
 
 
+def _guard_words(status, device):
+    if status.numel() < _lib.ST_WORDS or status.device != device:
+        raise ValueError("status: the %d words of a range guard on %s" % (_lib.ST_WORDS, device))
+    return _chk(status, torch.int32, "status")
+
+
 def grad_norm(grads, max_norm=float("inf"), grad_scale=1.0, out=None, counters=(), guard_range=True, status=None):
     """2-norm over all gradients of a list (GradList, a list of tensors, or a list of GradLists: one norm over all of them), on the
     device and without synchronising.  Returns float32 [4] = [norm of grad_scale * gradients, coefficient min(1, max_norm / (norm +
@@ -908,7 +920,7 @@ def grad_norm(grads, max_norm=float("inf"), grad_scale=1.0, out=None, counters=(
     at = words.data_ptr() if out is None else _norm_words(out, dev, "out")
     partials = torch.empty(room, dtype=torch.float64, device=dev)
     steps = (ctypes.c_void_p * len(counters))(*[_counter(c, dev) for c in counters]) if counters else None
-    guard = (mlp_status(dev) if status is None else status).data_ptr() if guard_range else None
+    guard = (lists[0].parts[0].guard if status is None else _guard_words(status, dev)) if guard_range else None
     stream = _stream()
     for g in lists:
         for part, _, _ in g.launches:
@@ -924,7 +936,7 @@ def adamw_count(step, norm=None, guard_range=True, status=None):
     if not step.is_cuda:
         _chk(step, name="step")
     with torch.cuda.device(dev):
-        guard = (mlp_status(dev) if status is None else status).data_ptr() if guard_range else None
+        guard = (mlp_status(dev).data_ptr() if status is None else _guard_words(status, dev)) if guard_range else None
         _lib.check(_lib.load().benerf_adamw_count(_counter(step, dev), None if norm is None else _norm_words(norm, dev, "norm"), guard, _stream()), "adamw_count")
 
 
@@ -954,7 +966,7 @@ def adamw_step(plan, grads, lr, step, betas=(0.9, 0.999), eps=1e-8, weight_decay
         lr_dev, lr = _counter(lr, dev), 0.0
     cfg = _lib.AdamwCfg(lr, betas[0], betas[1], eps, weight_decay, grad_scale, t or 0, int(seed) & 0xFFFFFFFFFFFFFFFF, lr_dev, step_dev)
     words = None if norm is None else _norm_words(norm, dev, "norm")
-    guard = (plan.guard if status is None else status.data_ptr()) if guard_range else None
+    guard = (plan.parts[0].guard if status is None else _guard_words(status, dev)) if guard_range else None
     stream = _stream()
     for part, kind, ptrs in launches:
         part.used_on(stream)

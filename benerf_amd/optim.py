@@ -327,7 +327,9 @@ class FusedAdamW(torch.optim.AdamW):
       master      float32 copies (state["master"]) of half-precision parameters: read and updated instead of them, rounded into them.
                   They are made from the parameters at the first step: weights that are loaded later need theirs dropped.
       capturable  counters live on the device, a step can be captured (make one step before, outside; learning rates that change need
-                  `lr` as a float32 tensor on the device).  With max_norm they live there too.
+                  `lr` as a float32 tensor on the device).  With max_norm they live there too.  A captured step goes on with the state,
+                  the counters and the set of gradients of its capture: load_state_dict, or a step outside with other gradients
+                  missing, needs a new capture.
       guard_range skip the step where the MLP's range guard says so, like FlatAdam.
     state[p]["step"] is ONE tensor for all parameters of a group that have made the same steps (state_dict gives each its own).
     amsgrad, maximize and differentiable are refused."""
@@ -340,6 +342,8 @@ class FusedAdamW(torch.optim.AdamW):
             raise ValueError("FusedAdamW: moments have 8 or 32 bits, not %r" % (state_bits,))
         if max_norm is not None and not max_norm > 0:
             raise ValueError("FusedAdamW: max_norm must be positive, got %r" % (max_norm,))
+        if kw.get("fused"):         # it would promise to undo a gradient scaler's factor
+            raise NotImplementedError("FusedAdamW: fused=True is torch's own kernel; leave it out")
         self._settings = dict(state_bits=state_bits, max_norm=max_norm, master=bool(master), seed=int(seed), guard_range=bool(guard_range))
         self._plans, self._states = {}, []
         self.grad_norm = None

@@ -96,6 +96,8 @@ def test_python_refusals():
     for kw in (dict(state_bits=16), dict(max_norm=0.0), dict(max_norm=-1.0), dict(max_norm=float("nan")), dict(weight_decay=-1.0), dict(lr=-1.0)):
         with pytest.raises(ValueError):
             optim.FusedAdamW([p], **kw)
+    with pytest.raises(NotImplementedError):
+        optim.FusedAdamW([p], fused=True)
     p.grad = torch.ones(4)
     with pytest.raises(_lib.BenerfHipError):
         optim.FusedAdamW([p]).step()

@@ -1,6 +1,7 @@
 """GPU: the optimiser operators over lists (K9) against a 64-bit evaluation (oracle/adamw_oracle.py): gradient norm with clip coefficient
 and verdict, AdamW with moments in 32 and 8 bits.  The bounds are the oracle's, counted in roundings; a rounding to bfloat16 is 2^-8 of the
 value, to float16 2^-11 (2^-25 below its normal range)."""
+import gc
 import math
 
 import numpy as np
@@ -398,12 +399,12 @@ def test_captured_step(K, bits):
     side = torch.cuda.CUDAGraph()
     with torch.cuda.graph(side):
         torch.zeros(1, device="cuda")
-        for call in (lambda: K.adamw_step(A.plan, sets[0][3], step=3, **HYPER), lambda: K.AdamWPlan(A.p, A.p, A.p)):
+        for call in (lambda: K.adamw_step(A.plan, sets[0][3], step=3, **HYPER), lambda: K.AdamWPlan(A.p, A.m, A.v), lambda: K.grad_norm(A.g)):
             try:
                 call()
             except (_lib.BenerfHipError, ValueError) as e:
                 refused.append(str(e))
-    assert len(refused) == 2 and "counter" in refused[0]
+    assert len(refused) == 3 and "counter" in refused[0] and "captured region" in refused[-1]
 
 
 def test_another_stream_and_the_plan_let_go(K):
@@ -423,6 +424,31 @@ def test_another_stream_and_the_plan_let_go(K):
         torch.cuda.current_stream().wait_stream(side)
         torch.cuda.synchronize()
         L.check(before)
+
+
+def test_a_captured_step_outlives_its_plan(K):
+    """A graph reads the plan's table at every replay, also after the caller has let plan and lists go."""
+    L = List(K, [3000, 33], seed=8, t=1)
+    step, words = torch.zeros((), device="cuda"), torch.zeros(4, device="cuda")
+    lists = [K.GradList(L.g, L.plan), K.GradList(L.g)]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        K.grad_norm(lists[1], 0.02, out=words, counters=[step])
+        K.adamw_step(L.plan, lists[0], step=step, norm=words, **HYPER)
+    tables = [part.dev_at for x in (L.plan, lists[1]) for part in x.parts]
+    assert all(at in K._captured for at in tables)
+    before = L.snapshot()
+    del L.plan, lists
+    gc.collect()
+    filled = [torch.full((256 << k,), 255, dtype=torch.uint8, device="cuda") for k in range(8) for _ in range(8)]
+    assert not any(x.data_ptr() in tables for x in filled)
+    _, coef = O.clip_words([_f64(g) for g in L.g], 0.02, 1.0)
+    for t in (1, 2, 3):
+        graph.replay()
+        torch.cuda.synchronize()
+        L.check(before, scale=coef, t=t)
+        before = L.snapshot()
+    assert float(step) == 3.0
 
 
 def test_same_result_every_time(K):
@@ -462,9 +488,14 @@ def test_refusals_on_the_device(K):
         from benerf_amd import _lib
         with pytest.raises(_lib.BenerfHipError):
             K.adamw_step(plan, g, 1e-3, **kw)
-    for kw in (dict(step=f(2)), dict(step=torch.zeros(1)), dict(step=1, norm=f(3))):
+    word = lambda n, d=torch.int32, **kw: torch.zeros(n, dtype=d, **dict(dict(device="cuda"), **kw))      # noqa: E731
+    for kw in (dict(step=f(2)), dict(step=torch.zeros(1)), dict(step=1, norm=f(3)), dict(step=1, status=word(15)), dict(step=1, status=word(16, device="cpu"))):
         with pytest.raises(ValueError):
             K.adamw_step(plan, g, 1e-3, **kw)
+    for call in (lambda **kw: K.grad_norm(g, 1.0, **kw), lambda **kw: K.adamw_count(f(1), **kw)):
+        for kw, error in ((dict(status=word(15)), ValueError), (dict(status=word(16, device="cpu")), ValueError), (dict(status=word(16, torch.float32)), TypeError)):
+            with pytest.raises(error):
+                call(**kw)
     with pytest.raises(ValueError):
         K.grad_norm(g, 1.0, out=f(3))
     with pytest.raises(TypeError):
