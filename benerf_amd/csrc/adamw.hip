@@ -47,6 +47,7 @@ struct Chunk {
     int32_t pad[3];
 };
 static_assert(sizeof(Chunk) == 80, "a multiple of 16 bytes");
+static_assert(sizeof(Chunk) >= BENERF_ST_WORDS * 4, "a record can be read in place of the guard's words");
 struct PlanHead {
     uint32_t magic;
     int32_t n_tensors;
@@ -88,10 +89,11 @@ struct AdamwArgs {
 };
 static_assert(sizeof(AdamwArgs) + sizeof(Ptrs<PTRS_LARGE>) <= 4096, "a launch's arguments");
 
+constexpr uint32_t GUARD_LIMIT = 0x477fe000u;       // 65504
 __device__ __forceinline__ bool guard_says_skip(const uint32_t* st) {
     if (!st) return false;
     const uint32_t skip = st[BENERF_ST_SKIP], act = st[BENERF_ST_ACT], grad = st[BENERF_ST_GRAD];
-    return skip != 0u || act >= 0x477fe000u || grad >= 0x477fe000u;
+    return (skip != 0u) | (act >= GUARD_LIMIT) | (grad >= GUARD_LIMIT);         // no word waits for another
 }
 
 __host__ __device__ inline double int_power(double b, int64_t t) {
@@ -117,12 +119,17 @@ __device__ __forceinline__ double reciprocal_root(double x) {
 // Scalars of this step; false: skipped.  What the host could not know (a counter or a learning rate on the device, steps skipped so
 // far) is worked out again here, in f64: 40 multiplications for t < 2^20, once per wave, uniform.
 __device__ __forceinline__ bool step_scalars(const AdamwArgs& a, Hyper& h, int64_t& t) {
-    // all words that may matter are read before any of them is looked at
-    const bool guard = guard_says_skip(a.status);
-    const uint32_t gated = a.status && !a.norm ? a.status[BENERF_ST_SKIPPED_TOTAL] : 0u;      // the norm's count holds them
-    const float coef = a.norm ? a.norm[1] : 1.f, verdict = a.norm ? a.norm[2] : 0.f, skipped = a.norm ? a.norm[3] : 0.f;
-    const float counted = a.step_dev ? a.step_dev[0] : 0.f, rate = a.lr_dev ? a.lr_dev[0] : 0.f;
-    if (guard || verdict != 0.f) return false;
+    // Every word that may matter is asked for at once, with the chunk's record, and before any is looked at; where there is none, the plan's
+    // records are read for it.  One word after the other: 30 values 3.9 us against 3.4, two networks 6.5 / 6.1, 4.8 M weights with 8-bit moments
+    // 18.8 / 17.8.
+    auto word = [&](const void* p, int i) { return static_cast<const uint32_t*>(p ? p : static_cast<const void*>(a.chunks))[i]; };
+    const uint32_t skip = word(a.status, BENERF_ST_SKIP), act = word(a.status, BENERF_ST_ACT), grad = word(a.status, BENERF_ST_GRAD), total = word(a.status, BENERF_ST_SKIPPED_TOTAL);
+    const uint32_t n1 = word(a.norm, 1), n2 = word(a.norm, 2), n3 = word(a.norm, 3), counter = word(a.step_dev, 0), rate_word = word(a.lr_dev, 0);
+    const bool guard = (a.status != nullptr) & ((skip != 0u) | (act >= GUARD_LIMIT) | (grad >= GUARD_LIMIT));
+    const uint32_t gated = a.status && !a.norm ? total : 0u;      // the norm's count holds them
+    const float coef = a.norm ? __uint_as_float(n1) : 1.f, verdict = a.norm ? __uint_as_float(n2) : 0.f, skipped = a.norm ? __uint_as_float(n3) : 0.f;
+    const float counted = __uint_as_float(counter), rate = __uint_as_float(rate_word);
+    if (guard | (verdict != 0.f)) return false;
     h = a.h;
     h.gs = h.gs * coef;
     t = a.step;
@@ -225,8 +232,8 @@ struct Four32 {
 
 // ---- moments in 8 bits -----------------------------------------------------------------------------------------------------------
 __device__ __forceinline__ float4v decode4(uint32_t w, float s) {
-    const auto a = __builtin_amdgcn_cvt_pk_f32_fp8(w, false), b = __builtin_amdgcn_cvt_pk_f32_fp8(w, true);
-    return float4v{a[0] * s, a[1] * s, b[0] * s, b[1] * s};
+    const auto a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w, s, false), b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w, s, true);
+    return float4v{a[0], a[1], b[0], b[1]};
 }
 __device__ __forceinline__ uint32_t pk_max(uint32_t a, uint32_t b) {
     typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
@@ -241,14 +248,14 @@ __device__ __forceinline__ uint32_t block_max(uint32_t x) {
     const auto r = __builtin_amdgcn_permlane16_swap(x, x, false, false);
     return pk_max(r[0], r[1]);
 }
-// |x| / scale on the e4m3 grid (steps of 2^(E - 3), 2^-9 from below 2^-6 on), down after the draw h / 2^16 is added: the draw goes into the
-// 20 bits behind the grid's three, which are then cut off - a carry is the step up.  Below 2^-6 the same happens 2^-6 higher up, where the
-// grid has the right step.  The scale is a power of two, so nothing else is rounded (but what 2^-6 + y loses: 2^-21 of a step).  inf and the
-// NaN of 0x7fc00000 come out as such, the conversion makes both NaN.
-__device__ __forceinline__ float to_grid(float x, float low, float inv, uint32_t h) {
-    const float c = x < low ? 1.f / 64.f : 0.f;
-    const uint32_t z = __float_as_uint(__builtin_fmaf(x, inv, c)) + (h << 4);
-    return __uint_as_float(z & 0xfff00000u) - c;
+// Four codes: x / scale on the e4m3 grid (steps of 2^(E - 3), 2^-9 from below 2^-6 on), down after the draw h / 2^16 of a step is added.  The
+// instruction puts the draw's 20 highest bits behind the grid's three and cuts them off, below 2^-6 too (compared with the formula in f64 for
+// 4 M values from 2^-24 to 2^8: no difference); inf becomes NaN.  213 vector instructions a wavefront against 277 without it: 4.3 M weights 13.6 -> 12.8 us.
+__device__ __forceinline__ uint32_t codes4(float4v x, float scale, const uint32_t (&h)[4]) {
+    int w = __builtin_amdgcn_cvt_scalef32_sr_fp8_f32(0, x[0], h[0], scale, 0);
+    w = __builtin_amdgcn_cvt_scalef32_sr_fp8_f32(w, x[1], h[1], scale, 1);
+    w = __builtin_amdgcn_cvt_scalef32_sr_fp8_f32(w, x[2], h[2], scale, 2);
+    return (uint32_t)__builtin_amdgcn_cvt_scalef32_sr_fp8_f32(w, x[3], h[3], scale, 3);
 }
 template <bool PAST>
 __device__ __forceinline__ uint32_t load_codes(const void* p, int i, int k) {
@@ -345,20 +352,13 @@ struct Four8 {
         const uint32_t em = max(top >> 23, 27u), eu = max(top >> 7 & 0xffu, 27u);
         ms = __uint_as_float((em - 7u) << 23);
         us = __uint_as_float((eu - 7u) << 23);
-        const float im = __uint_as_float((261u - em) << 23), iu = __uint_as_float((261u - eu) << 23);
-        const float lm = __uint_as_float((em - 13u) << 23), lu = __uint_as_float((eu - 13u) << 23), least = __uint_as_float((eu - 16u) << 23);
+        const float least = __uint_as_float((eu - 16u) << 23);
         const uint4 r = draws4(group, t, key);
-        const uint32_t rw[4] = {r.x, r.y, r.z, r.w};
-        float a[4], b[4];
+        // one step is the least that a root above 0 may become: lifted to it, it stays there whatever the draw
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            a[j] = copysignf(to_grid(fabsf(m[j]), lm, im, rw[j] & 0xffffu), m[j]);
-            // one step is the least that a value above 0 may become: lifted to it, it stays there whatever the draw
-            const float lifted = root[j] < least ? (v[j] > 0.f ? least : 0.f) : root[j];
-            b[j] = to_grid(lifted, lu, iu, rw[j] >> 16);
-        }
-        mw = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(a[2], a[3], __builtin_amdgcn_cvt_pk_fp8_f32(a[0], a[1], 0, false), true);
-        uw = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(b[2], b[3], __builtin_amdgcn_cvt_pk_fp8_f32(b[0], b[1], 0, false), true);
+        for (int j = 0; j < 4; ++j) root[j] = root[j] < least ? (v[j] > 0.f ? least : 0.f) : root[j];
+        mw = codes4(m, ms, {r.x << 16, r.y << 16, r.z << 16, r.w << 16});
+        uw = codes4(root, us, {r.x & 0xffff0000u, r.y & 0xffff0000u, r.z & 0xffff0000u, r.w & 0xffff0000u});
     }
     __device__ __forceinline__ void store(const Chunk& c, int i, int k) const {
         if (MASTER) F32::store<PAST>(c.master, i, k, w);
@@ -385,10 +385,10 @@ __device__ __forceinline__ uint32_t chunk_of(uint32_t b, uint32_t n) {
 // One workgroup per chunk, four elements a thread.
 template <class PT, class GT, int BITS, bool MASTER, int N, bool PAST>
 __global__ __launch_bounds__(THREADS) void adamw_kernel(AdamwArgs a, Ptrs<N> grads) {
+    const Chunk c = a.chunks[chunk_of(blockIdx.x, gridDim.x)];
     Hyper h;
     int64_t t;
     const bool go = step_scalars(a, h, t);
-    const Chunk c = a.chunks[chunk_of(blockIdx.x, gridDim.x)];
     const char* gp = static_cast<const char*>(grads.p[c.tensor - a.tensor0]);
     if (!gp || !go) return;
     gp += (int64_t)c.index * CHUNK * GT::BYTES;
