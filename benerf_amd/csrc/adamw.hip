@@ -651,7 +651,7 @@ extern "C" int benerf_adamw_plan_fill(const BenerfAdamwTensor* tensors_host, int
                            (((uintptr_t)t.exp_avg_scale | (uintptr_t)t.exp_avg_sq_scale) & 3) == 0,
                        "adamw_plan_fill: tensor %d is not aligned to its elements", k);
     }
-    memset(plan_host, 0, need);
+    memset(plan_host, 0, HEAD_BYTES);
     PlanHead* h = static_cast<PlanHead*>(plan_host);
     h->magic = PLAN_MAGIC;
     h->n_tensors = n_tensors;
@@ -672,6 +672,7 @@ extern "C" int benerf_adamw_plan_fill(const BenerfAdamwTensor* tensors_host, int
         e[k] = Entry{t.n, at};
         for (int64_t i = 0; i < t.n; i += CHUNK, ++at, ++chunk) {
             const int64_t w = state_bits == 8 ? 1 : 4;
+            memset(chunk, 0, sizeof(Chunk));
             chunk->param = on(t.param, i * type_bytes(param_type));
             chunk->m = on(t.exp_avg, i * w);
             chunk->v = on(t.exp_avg_sq, i * w);

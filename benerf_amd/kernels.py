@@ -4,6 +4,8 @@ Every wrapper validates dtype / device / contiguity and raises on any non-zero r
 """
 import array
 import ctypes
+import itertools
+import operator
 import os
 
 import torch
@@ -714,6 +716,18 @@ def _list_tensor(t, name, device, dtypes, numel=None):
 _captured = {}                      # plans' tables that captured launches read at every replay: never freed
 
 
+_address, _numel, _dtype, _detach = torch.Tensor.data_ptr, torch.Tensor.numel, operator.attrgetter("dtype"), torch.Tensor.detach
+
+
+def _list_tensors(ts, name, device, dtypes, numels=None):
+    """_list_tensor over a list, through map() where nothing is wrong with it; numels None: any."""
+    if (device is not None and device.type == "cuda" and all(map(torch.is_tensor, ts)) and set(map(_dtype, ts)) <= set(dtypes) and
+            set(map(torch.Tensor.get_device, ts)) == {device.index} and all(map(torch.Tensor.is_contiguous, ts)) and
+            (numels is None or list(map(_numel, ts)) == numels)):
+        return list(map(_detach, ts))
+    return [_list_tensor(t, "%s %d" % (name, k), device, dtypes, None if numels is None else numels[k]) for k, t in enumerate(ts)]
+
+
 class _Part:
     """The tensors of one element type in a list, and their plan: the host copy and the one on the device."""
 
@@ -727,12 +741,12 @@ class _Part:
         size = lib.benerf_adamw_plan_bytes(table, n)
         if size == 0:
             raise ValueError("a tensor of the list is too large")
-        whole = ctypes.create_string_buffer(size)
-        _lib.check(lib.benerf_adamw_plan_fill(table, n, param_type, state_bits, whole, size), "adamw_plan_fill")
-        self.host = ctypes.create_string_buffer(bytes(memoryview(whole)[:64 + 16 * n]))      # what calls read of it
+        whole = torch.empty(size, dtype=torch.uint8, device="cpu")
+        _lib.check(lib.benerf_adamw_plan_fill(table, n, param_type, state_bits, whole.data_ptr(), size), "adamw_plan_fill")
+        self.host = ctypes.create_string_buffer(ctypes.string_at(whole.data_ptr(), 64 + 16 * n))      # what calls read of it
         with torch.cuda.device(device):
             # a blocking copy: the plan is there before anything is queued on any stream
-            self.dev = torch.frombuffer(whole, dtype=torch.uint8).to(device)
+            self.dev = whole.to(device)
             self.stream = _stream()
         self.host_at, self.dev_at = ctypes.addressof(self.host), self.dev.data_ptr()
         self.partials = int(lib.benerf_grad_norm_partials(self.host))
@@ -758,14 +772,18 @@ class GradList:
         self.device = plan.device if plan is not None else next((t.device for t in tensors if torch.is_tensor(t)), None)
         if self.device is None:
             raise ValueError("GradList: no gradient in the list")
-        self.tensors = [None if t is None else
-                        _list_tensor(t, "gradient %d" % k, self.device, tuple(_ELEMENT_TYPES), None if plan is None else plan.numels[k])
-                        for k, t in enumerate(tensors)]
+        if not any(t is None for t in tensors):
+            self.tensors = _list_tensors(tensors, "gradient", self.device, tuple(_ELEMENT_TYPES), None if plan is None else plan.numels)
+        else:
+            self.tensors = [None if t is None else
+                            _list_tensor(t, "gradient %d" % k, self.device, tuple(_ELEMENT_TYPES), None if plan is None else plan.numels[k])
+                            for k, t in enumerate(tensors)]
         if plan is not None:
             self.parts = plan.parts
         else:
             kind = next(t.dtype for t in self.tensors if t is not None)
-            self.parts = [_Part(range(len(tensors)), [_lib.AdamwTensor(n=0 if t is None else t.numel()) for t in self.tensors], _ELEMENT_TYPES[kind], 0, self.device)]
+            rows = [(None,) * 6 + (0 if t is None else t.numel(), 0) for t in self.tensors]
+            self.parts = [_Part(range(len(tensors)), rows, _ELEMENT_TYPES[kind], 0, self.device)]
         self._bind()
 
     @classmethod
@@ -797,10 +815,10 @@ def _grad_launches(parts, tensors):
     return out
 
 
-def _no_overlap(lists):
-    """Refuses tensors that share memory: two workgroups would write the same elements."""
-    spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for l in lists if l is not None for t in l if t is not None and t.numel())
-    if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
+def _no_overlap(spans):
+    """Refuses tensors that share memory: two workgroups would write the same elements.  spans: (first, past the last) byte of each."""
+    spans = sorted(spans)
+    if any(map(operator.gt, map(operator.itemgetter(1), spans), map(operator.itemgetter(0), spans[1:]))):
         raise ValueError("two tensors of the list share memory (the same tensor twice?)")
 
 
@@ -821,15 +839,15 @@ class AdamWPlan:
         if n == 0:
             raise ValueError("AdamWPlan: empty list")
         self.device = params[0].device if torch.is_tensor(params[0]) else None
-        self.params = [_list_tensor(p, "parameter %d" % k, self.device, tuple(_ELEMENT_TYPES)) for k, p in enumerate(params)]
-        self.numels = [p.numel() for p in self.params]
+        self.params = _list_tensors(params, "parameter", self.device, tuple(_ELEMENT_TYPES))
+        self.numels = list(map(_numel, self.params))
+        blocks = [-(-m // ADAMW_BLOCK) for m in self.numels]
 
-        def like(ts, name, dtype, blocks=False):
+        def like(ts, name, dtype, sizes=self.numels):
             ts = list(ts)
             if len(ts) != n:
                 raise ValueError("%s: %d tensors for %d parameters" % (name, len(ts), n))
-            return [_list_tensor(t, "%s %d" % (name, k), self.device, (dtype,), -(-self.numels[k] // ADAMW_BLOCK) if blocks else self.numels[k])
-                    for k, t in enumerate(ts)]
+            return _list_tensors(ts, name, self.device, (dtype,), sizes)
         exp_avg, exp_avg_sq = list(exp_avg), list(exp_avg_sq)
         self.state_bits = 8 if exp_avg and torch.is_tensor(exp_avg[0]) and exp_avg[0].dtype == CODE_TYPE else 32
         if (self.state_bits == 8) != (exp_avg_scale is not None) or (self.state_bits == 8) != (exp_avg_sq_scale is not None):
@@ -838,8 +856,8 @@ class AdamWPlan:
         self.exp_avg, self.exp_avg_sq = like(exp_avg, "exp_avg", kind), like(exp_avg_sq, "exp_avg_sq", kind)
         self.exp_avg_scale = self.exp_avg_sq_scale = None
         if self.state_bits == 8:
-            self.exp_avg_scale = like(exp_avg_scale, "exp_avg_scale", torch.float32, True)
-            self.exp_avg_sq_scale = like(exp_avg_sq_scale, "exp_avg_sq_scale", torch.float32, True)
+            self.exp_avg_scale = like(exp_avg_scale, "exp_avg_scale", torch.float32, blocks)
+            self.exp_avg_sq_scale = like(exp_avg_sq_scale, "exp_avg_sq_scale", torch.float32, blocks)
         self.master = None
         if master is not None:
             master = list(master)
@@ -853,14 +871,15 @@ class AdamWPlan:
                     self.master.append(None)
                 else:
                     self.master.append(_list_tensor(t, "master %d" % k, self.device, (torch.float32,), self.numels[k]))
-        _no_overlap([self.params, self.exp_avg, self.exp_avg_sq, self.exp_avg_scale, self.exp_avg_sq_scale, self.master])
-        at = lambda l, k: None if l is None or l[k] is None else l[k].data_ptr()       # noqa: E731
-        rows, block = {}, 0
-        for k, p in enumerate(self.params):
-            rows.setdefault(p.dtype, []).append((k, _lib.AdamwTensor(
-                param=p.data_ptr(), exp_avg=at(self.exp_avg, k), exp_avg_sq=at(self.exp_avg_sq, k), exp_avg_scale=at(self.exp_avg_scale, k),
-                exp_avg_sq_scale=at(self.exp_avg_sq_scale, k), master=at(self.master, k), n=p.numel(), first_block=block)))
-            block += -(-p.numel() // ADAMW_BLOCK)
+        # addresses of the six kinds of tensor, list by list, None where there is none
+        lists = (self.params, self.exp_avg, self.exp_avg_sq, self.exp_avg_scale, self.exp_avg_sq_scale, self.master)
+        at = [[None] * n if l is None else [None if t is None else _address(t) for t in l] for l in lists]
+        widths = [[p.element_size() for p in self.params]] + [[1 if self.state_bits == 8 else 4] * n] * 2 + [[4] * n] * 3
+        _no_overlap((a, a + m * w) for l, ws, ms in zip(at, widths, (self.numels,) * 3 + (blocks,) * 2 + (self.numels,)) for a, w, m in zip(l, ws, ms)
+                    if a is not None and m)
+        rows = {}
+        for k, (p, row) in enumerate(zip(self.params, zip(*at, self.numels, itertools.accumulate(blocks, initial=0)))):
+            rows.setdefault(p.dtype, []).append((k, row))
         self.parts = [_Part([k for k, _ in r], [x for _, x in r], _ELEMENT_TYPES[d], self.state_bits, self.device) for d, r in rows.items()]
 
 
