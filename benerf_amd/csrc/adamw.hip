@@ -24,6 +24,7 @@ constexpr int THREADS = 128;
 constexpr int BLOCK = BENERF_ADAMW_BLOCK;
 constexpr int CHUNK = THREADS * 4;           // elements a workgroup of the step takes: four a thread
 constexpr int64_t PAST_BYTES = 320ll << 20;  // see Shape
+constexpr int64_t MAX_CHUNKS = 1ll << 24;    // of a list: a grid holds 2^32 threads
 constexpr uint32_t PLAN_MAGIC = 0x41445731u;
 static_assert(BLOCK == 128, "a block is half a wavefront of four elements a lane");
 
@@ -624,7 +625,8 @@ extern "C" size_t benerf_adamw_plan_bytes(const BenerfAdamwTensor* tensors_host,
     if (!tensors_host || n_tensors <= 0) return 0;
     for (int k = 0; k < n_tensors; ++k)
         if (tensors_host[k].n < 0 || tensors_host[k].n > (1ll << 40)) return 0;
-    return HEAD_BYTES + sizeof(Entry) * (size_t)n_tensors + sizeof(Chunk) * (size_t)count_chunks(tensors_host, n_tensors);
+    const int64_t chunks = count_chunks(tensors_host, n_tensors);
+    return chunks < MAX_CHUNKS ? HEAD_BYTES + sizeof(Entry) * (size_t)n_tensors + sizeof(Chunk) * (size_t)chunks : 0;
 }
 
 extern "C" int benerf_adamw_plan_fill(const BenerfAdamwTensor* tensors_host, int n_tensors, int param_type, int state_bits, void* plan_host, size_t plan_bytes) {
@@ -632,7 +634,7 @@ extern "C" int benerf_adamw_plan_fill(const BenerfAdamwTensor* tensors_host, int
     BENERF_REQUIRE(param_type >= BENERF_F32 && param_type <= BENERF_F16, "adamw_plan_fill: unknown parameter type %d", param_type);
     BENERF_REQUIRE(state_bits == 0 || state_bits == 8 || state_bits == 32, "adamw_plan_fill: moments have 8 or 32 bits (0: gradients only), not %d", state_bits);
     const size_t need = benerf_adamw_plan_bytes(tensors_host, n_tensors);
-    BENERF_REQUIRE(need != 0, "adamw_plan_fill: a tensor's size is negative or beyond 2^40");
+    BENERF_REQUIRE(need != 0, "adamw_plan_fill: a tensor's size is negative, or the list has 2^24 chunks of 512 elements or more");
     if (plan_bytes < need) {
         benerf_set_error("adamw_plan_fill: %zu bytes, %zu needed", plan_bytes, need);
         return BENERF_EWORKSPACE;
@@ -662,7 +664,6 @@ extern "C" int benerf_adamw_plan_fill(const BenerfAdamwTensor* tensors_host, int
     h->n_chunks = count_chunks(tensors_host, n_tensors);
     h->chunks_at = (int64_t)(HEAD_BYTES + sizeof(Entry) * (size_t)n_tensors);
     h->bytes = (int64_t)need;
-    BENERF_REQUIRE(h->n_chunks < (1ll << 24), "adamw_plan_fill: more than 2^24 chunks of 512 elements");      // a grid holds 2^32 threads
     Entry* e = reinterpret_cast<Entry*>(static_cast<char*>(plan_host) + HEAD_BYTES);
     Chunk* chunk = reinterpret_cast<Chunk*>(static_cast<char*>(plan_host) + h->chunks_at);
     int64_t at = 0;

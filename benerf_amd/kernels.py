@@ -740,7 +740,7 @@ class _Part:
         table = (_lib.AdamwTensor * n)(*rows)
         size = lib.benerf_adamw_plan_bytes(table, n)
         if size == 0:
-            raise ValueError("a tensor of the list is too large")
+            raise ValueError("the list is too large: 2^24 pieces of 512 elements or more")
         whole = torch.empty(size, dtype=torch.uint8, device="cpu")
         _lib.check(lib.benerf_adamw_plan_fill(table, n, param_type, state_bits, whole.data_ptr(), size), "adamw_plan_fill")
         self.host = ctypes.create_string_buffer(ctypes.string_at(whole.data_ptr(), 64 + 16 * n))      # what calls read of it

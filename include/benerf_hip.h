@@ -418,7 +418,7 @@ int benerf_adam_step(float* param, const float* grad, float* exp_avg, float* exp
  *   first_block: number of the tensor's first block of 128 in the caller's numbering (8 bits: the generator's counter; give every
  *                tensor its own range).
  * Element types of parameters and gradients: BENERF_F32 / _BF16 / _F16, one of each per plan / call.  Pointers need the alignment of
- * an element.  n = 0 is allowed. */
+ * an element.  n = 0 is allowed; a list has fewer than 2^24 pieces of 512 elements (8.6e9 elements), every tensor's last one counted whole. */
 enum { BENERF_F32 = 0, BENERF_BF16 = 1, BENERF_F16 = 2 };
 enum { BENERF_ADAMW_BLOCK = 128 };
 typedef struct BenerfAdamwTensor {

@@ -32,6 +32,8 @@ def test_plan_sizes(lib):
     # header 64, 16 bytes a tensor, 80 bytes a chunk of 512 elements
     size = lambda *ns: lib.benerf_adamw_plan_bytes(_rows(*ns), len(ns))      # noqa: E731
     assert size(1) == 64 + 16 + 80 and size(512, 513, 0) == 64 + 3 * 16 + 80 * 3 and size(1 << 30) == 64 + 16 + (80 << 21)
+    # fewer than 2^24 chunks in all
+    assert size((1 << 33) - 512) == 64 + 16 + 80 * ((1 << 24) - 1) and size((1 << 33) - 511) == 0 and size(1 << 32, 1 << 32) == 0 and size(*[1 << 40] * 64) == 0
     assert size(-1) == 0 and size(1 << 41) == 0 and lib.benerf_adamw_plan_bytes(None, 1) == 0
 
 
