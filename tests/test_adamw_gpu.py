@@ -451,6 +451,34 @@ def test_a_captured_step_outlives_its_plan(K):
     assert float(step) == 3.0
 
 
+@pytest.mark.parametrize("sizes", [[300, 7], [200000, 33], [1000] * 70])
+def test_norms_at_once(K, sizes):
+    """Two graphs over one list, replayed on two streams beside an eager call on a third: nobody's sums reach another's words."""
+    gen = torch.Generator().manual_seed(4)
+    g = [torch.randn(n, generator=gen).cuda() for n in sizes]
+    grads = K.GradList(g)
+    want = [O.clip_words([_f64(x) for x in g], 1.0, scale)[0] for scale in (1.0, 2.0, 3.0)]
+    K.grad_norm(grads)
+    graphs, words = [torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()], [torch.zeros(4, device="cuda") for _ in range(3)]
+    for graph, w, scale in zip(graphs, words, (1.0, 2.0)):
+        with torch.cuda.graph(graph):
+            K.grad_norm(grads, 1.0, scale, out=w)
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    for it in range(4):
+        for w in words:
+            w.zero_()
+        torch.cuda.synchronize()
+        for _ in range(5):
+            for stream, graph in zip(streams, graphs):
+                with torch.cuda.stream(stream):
+                    graph.replay()
+            with torch.cuda.stream(streams[2]):
+                K.grad_norm(grads, 1.0, 3.0, out=words[2])
+        torch.cuda.synchronize()
+        for w, norm in zip(words, want):
+            assert abs(float(w[0]) - norm) <= 2 * O.HALF * norm and w[2:].tolist() == [0.0, 0.0]
+
+
 def test_same_result_every_time(K):
     """No order of atomics, no leftover: the same inputs give the same bits, seeds give other roundings."""
     def once(seed):

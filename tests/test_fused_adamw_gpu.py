@@ -229,10 +229,10 @@ def test_closure_hooks_deepcopy_and_refusals(optim):
         return loss
     o.register_step_pre_hook(lambda *a: calls.append("pre"))
     o.register_step_post_hook(lambda *a: calls.append("post"))
-    first = float(o.step(closure))
-    for _ in range(30):
-        last = float(o.step(closure))
-    assert last < first and calls[:2] == ["pre", "post"] and len(calls) == 62
+    for _ in range(31):
+        want = float((ps[0].detach() ** 2).sum())
+        assert float(o.step(closure)) == want
+    assert calls[:2] == ["pre", "post"] and len(calls) == 62
     sched = torch.optim.lr_scheduler.StepLR(o, 1, 0.5)
     o.step(closure)
     sched.step()
@@ -257,6 +257,33 @@ def test_closure_hooks_deepcopy_and_refusals(optim):
     strided.grad = torch.ones_like(strided)
     with pytest.raises(ValueError):
         optim.FusedAdamW([strided]).step()
+
+
+def test_under_a_gradient_scaler(optim):
+    """Factors that are powers of two change nothing; a gradient that overflowed skips the step, its moments and its counter."""
+    plain, scaled = _params([(40, 5), (3,)]), _params([(40, 5), (3,)])
+    a, b = optim.FusedAdamW(plain, max_norm=0.5), optim.FusedAdamW(scaled, max_norm=0.5)
+    scaler = torch.amp.GradScaler("cuda", init_scale=1024.0, growth_interval=1000)
+    x = torch.randn(16, 40, generator=torch.Generator().manual_seed(1)).cuda()
+
+    def loss(ps, factor=1.0):
+        return ((x @ ps[0]).square().mean() + ps[1].square().sum()) * factor
+    for it in range(5):
+        if it == 2:
+            before = [p.detach().clone() for p in scaled]
+            scaler.scale(loss(scaled, 1e38)).backward()
+            scaler.step(b)
+            scaler.update()
+            b.zero_grad()
+            assert all(torch.equal(p, q) for p, q in zip(scaled, before)) and scaler.get_scale() == 512.0 and float(b.state[scaled[0]]["step"]) == 2.0
+        loss(plain).backward()
+        a.step()
+        a.zero_grad()
+        scaler.scale(loss(scaled)).backward()
+        scaler.step(b)
+        scaler.update()
+        b.zero_grad()
+        assert all(torch.equal(p, q) for p, q in zip(plain, scaled))
 
 
 @pytest.mark.parametrize("bits,clip", [(32, None), (8, 0.2)])
