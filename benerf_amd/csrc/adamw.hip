@@ -388,7 +388,7 @@ __device__ __forceinline__ uint32_t chunk_of(uint32_t b, uint32_t n) {
 // One workgroup per chunk, four elements a thread: wide loads, 38 registers, all 32 wavefronts a CU.  Long lists are bound by HBM - 126 M bfloat16
 // with master copies 570 us (6.2 TB/s), 235 M with 8-bit moments 577 (6.6) -, short ones by the launch and the way to the data, kernel
 // arguments, then record and words, then the gradient's address: 3.4 us for 30 values, 6.1 for two networks of 1.2 M (5.5 TB/s).  Four and eight chunks
-// in a row to a workgroup: 639 / 667, 654 / 664 and 9.9 / 13.6 us.
+// in a row to a workgroup: 639 / 667, 654 / 664 and 9.9 / 13.6 us; workgroups and chunks half and twice as large: 585 / 581, 592 / 599, 6.1 / 6.2.
 template <class PT, class GT, int BITS, bool MASTER, int N, bool PAST>
 __global__ __launch_bounds__(THREADS) void adamw_kernel(AdamwArgs a, Ptrs<N> grads) {
     const Chunk c = a.chunks[chunk_of(blockIdx.x, gridDim.x)];
