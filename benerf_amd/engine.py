@@ -663,8 +663,9 @@ class TrainStep:
                         self.net_steps.fill_(float(st["step"]))
                         continue
                     off -= self.off_moments
-                    self.flat_m[off:off + n].copy_(st["exp_avg"].reshape(-1))
-                    self.flat_v[off:off + n].copy_(st["exp_avg_sq"].reshape(-1))
+                    held = optim.convert_moments(st, 32)        # a checkpoint of AdamW in 8 bits holds codes, those of v's ROOT
+                    self.flat_m[off:off + n].copy_(held["exp_avg"].reshape(-1))
+                    self.flat_v[off:off + n].copy_(held["exp_avg_sq"].reshape(-1))
                     if "step" in st:
                         a_ = int(float(st["step"]))
                         applied = a_ if applied is None else max(applied, a_)
