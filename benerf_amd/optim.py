@@ -257,6 +257,8 @@ def zero_moments(params, bits):
 def convert_moments(state, bits):
     """A parameter's saved moments in the form that `bits` asks for, as a new dict of the tensors zero_moments names."""
     coded = "exp_avg_scale" in state
+    if not coded and state["exp_avg"].dtype == K.CODE_TYPE:
+        raise ValueError("8-bit moments without their scales")
     if coded == (bits == 8):
         return {k: state[k] for k in ("exp_avg", "exp_avg_sq") + (("exp_avg_scale", "exp_avg_sq_scale") if coded else ())}
     if coded:
@@ -292,21 +294,31 @@ _address, _numel, _device, _contiguous = torch.Tensor.data_ptr, torch.Tensor.num
 
 
 class _Group:
-    """What a step needs of one parameter group, made once and again when something was replaced or moved."""
-    PARTS = itemgetter("exp_avg", "exp_avg_sq", "step")
+    """What a step needs of one parameter group, made once and again when something was replaced, dropped or moved."""
+    MASTER = itemgetter("master")
 
     def __init__(self, params, plan, states, cohorts, on_device):
         self.params, self.plan, self.states, self.cohorts, self.on_device = params, plan, states, cohorts, on_device
         self.at = list(map(_address, params))
+        self.kinds = itemgetter("exp_avg", "exp_avg_sq", "step", *(("exp_avg_scale", "exp_avg_sq_scale") if plan.state_bits == 8 else ()))
+        self.with_master = [st for st, x in zip(states, plan.master or ()) if x is not None]
         self.look()
 
+    def watched(self):
+        """Every tensor of state that the plan or a counter stands for."""
+        return itertools.chain(itertools.chain.from_iterable(map(self.kinds, self.states)), map(self.MASTER, self.with_master))
+
     def look(self):
-        self.parts = list(itertools.chain.from_iterable(map(self.PARTS, self.states)))
+        self.parts = list(self.watched())
 
     def holds(self, params):
         """Parameters, their addresses and their state are the ones that the plan was made for."""
-        return (len(params) == len(self.params) and all(map(is_, params, self.params)) and list(map(_address, params)) == self.at and
-                all(map(is_, itertools.chain.from_iterable(map(self.PARTS, self.states)), self.parts)))
+        if len(params) != len(self.params) or not all(map(is_, params, self.params)) or list(map(_address, params)) != self.at:
+            return False
+        try:
+            return all(map(is_, self.watched(), self.parts))
+        except KeyError:            # a dropped one
+            return False
 
 
 def _hooks_or_profiler():
@@ -317,7 +329,8 @@ class FusedAdamW(torch.optim.AdamW):
     """torch.optim.AdamW (decoupled weight decay; same param_groups, state and state_dict) whose step() is one K9 launch per group.
 
     Parameters stay where they are: float32, bfloat16 or float16, contiguous, on one device.  A parameter without a gradient is left
-    alone, with its moments and its counter; a parameter that has moved (`p.data = ...`) is followed.
+    alone, with its moments and its counter; a parameter that has moved (`p.data = ...`) is followed, and so is a tensor of state that was
+    assigned or dropped.
       state_bits  32: exp_avg, exp_avg_sq in float32, whatever the parameter's type.  8: exp_avg in float8_e4m3fn and exp_avg_sq as the
                   float8_e4m3fn codes of its ROOT, exp_avg_scale and exp_avg_sq_scale with a float32 for every 128 elements, rounded
                   stochastically with `seed` (16.1 instead of 28 bytes of traffic and 2.1 instead of 8 of memory per parameter).
@@ -325,7 +338,8 @@ class FusedAdamW(torch.optim.AdamW):
       max_norm    None, or the global 2-norm over ALL groups to which gradients are clipped in the same step; a norm that is not finite
                   skips the step on the device.  After step(), grad_norm holds [norm, coefficient, skipped?, steps skipped so far].
       master      float32 copies (state["master"]) of half-precision parameters: read and updated instead of them, rounded into them.
-                  They are made from the parameters at the first step: weights that are loaded later need theirs dropped.
+                  They are made from the parameters at the first step: weights that are loaded later need theirs dropped
+                  (`del opt.state[p]["master"]`), the next step makes them again.
       capturable  counters live on the device, a step can be captured (make one step before, outside; learning rates that change need
                   `lr` as a float32 tensor on the device).  With max_norm they live there too.  A captured step goes on with the state,
                   the counters and the set of gradients of its capture: load_state_dict, or a step outside with other gradients

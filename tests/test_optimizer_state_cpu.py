@@ -1,6 +1,7 @@
 """CPU: what becomes of optimiser state outside the kernels - checkpoints of one form read by the other - with the real host code on host tensors."""
 from types import SimpleNamespace
 
+import pytest
 import torch
 
 LR = 5e-4
@@ -68,3 +69,89 @@ def test_eight_bit_checkpoint_into_a_train_step():
             assert torch.equal(step.flat_m[305 - step.off_moments:], torch.full((24,), 0.5)) and torch.equal(step.flat_v[305 - step.off_moments:], torch.full((24,), 0.25))
             assert step.global_step == 9 and int(step.guard.words[12]) == 2
             assert net_bits is None or float(step.net_steps) == 7.0
+
+
+class _Plan:
+    """Stands for kernels.AdamWPlan on the host: remembers what it was made of."""
+    made = []
+
+    def __init__(self, params, exp_avg, exp_avg_sq, exp_avg_scale=None, exp_avg_sq_scale=None, master=None):
+        self.params, self.numels, self.device, self.parts = params, [p.numel() for p in params], SimpleNamespace(index=-1), []
+        self.state_bits, self.master = 32 if exp_avg_scale is None else 8, master
+        self.held = dict(exp_avg=exp_avg, exp_avg_sq=exp_avg_sq, exp_avg_scale=exp_avg_scale, exp_avg_sq_scale=exp_avg_sq_scale, master=master)
+        _Plan.made.append(self)
+
+
+@pytest.fixture
+def plans(monkeypatch):
+    """FusedAdamW without a GPU: plans are _Plan, a step marks what it would write (masters + 1, rounded into their parameters)."""
+    from benerf_amd import kernels as K
+    _Plan.made = []
+
+    def step(plan, grads, *a, **kw):
+        for k, p in enumerate(plan.params):
+            x = plan.held["master"][k] if plan.held["master"] else None
+            (p if x is None else x).add_(1.0)
+            if x is not None:
+                p.copy_(x)
+    monkeypatch.setattr(K, "AdamWPlan", _Plan)
+    monkeypatch.setattr(K.GradList, "of_checked", classmethod(lambda cls, grads, plan: grads))
+    monkeypatch.setattr(K, "adamw_step", step)
+    return _Plan.made
+
+
+def _steps(opt, params, n=1):
+    for _ in range(n):
+        for p in params:
+            p.grad = torch.ones_like(p)
+        opt.step()
+
+
+def test_dropped_and_assigned_masters_are_followed(plans):
+    """Weights loaded in place after a step and their masters dropped: the next step starts from the loaded weights and there are masters again; an
+    assigned master is the one that is read and written; without either the plan stays."""
+    from benerf_amd import optim
+    params = [torch.nn.Parameter(torch.zeros(5, dtype=torch.bfloat16)), torch.nn.Parameter(torch.zeros(3)), torch.nn.Parameter(torch.zeros(4, dtype=torch.float16))]
+    opt = optim.FusedAdamW(params, master=True)
+    _steps(opt, params, 3)
+    assert len(plans) == 1 and all(torch.equal(p, torch.full_like(p, 3.0)) for p in params) and "master" not in opt.state[params[1]]
+    with torch.no_grad():
+        for p in params:
+            p.fill_(8.0)
+    for p in (params[0], params[2]):
+        del opt.state[p]["master"]
+    _steps(opt, params)
+    assert all(torch.equal(p, torch.full_like(p, 9.0)) for p in params), params
+    assert all(torch.equal(opt.state[p]["master"], torch.full(p.shape, 9.0)) for p in (params[0], params[2])) and len(plans) == 2
+    assert float(opt.state[params[0]]["step"]) == 4.0
+    mine = torch.full((4,), 20.0)
+    opt.state[params[2]]["master"] = mine
+    _steps(opt, params, 2)
+    assert torch.equal(mine, torch.full((4,), 22.0)) and torch.equal(params[2], torch.full_like(params[2], 22.0)) and len(plans) == 3
+    assert "master" in opt.state_dict()["state"][0]
+
+
+def test_dropped_and_assigned_moments_are_followed(plans):
+    """Codes, scales and counters that are assigned are the ones of the next step; moments that are dropped start at zero, codes without their
+    scales are refused."""
+    from benerf_amd import optim
+    params = [torch.nn.Parameter(torch.zeros(300)), torch.nn.Parameter(torch.zeros(5))]
+    opt = optim.FusedAdamW(params, state_bits=8)
+    _steps(opt, params, 2)
+    assert len(plans) == 1
+    for count, name in enumerate(("exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale", "step"), 2):
+        opt.state[params[0]][name] = opt.state[params[0]][name].clone()
+        _steps(opt, params, 2)
+        assert len(plans) == count, name
+        if name != "step":
+            assert plans[-1].held[name][0] is opt.state[params[0]][name]
+    st = opt.state[params[1]]
+    for name in ("exp_avg", "exp_avg_scale", "exp_avg_sq", "exp_avg_sq_scale"):
+        del st[name]
+    _steps(opt, params)
+    assert plans[-1].held["exp_avg_scale"][1] is st["exp_avg_scale"] and not st["exp_avg"].float().any() and float(st["step"]) == 13.0
+    del st["exp_avg_sq_scale"], st["exp_avg_scale"]
+    for p in params:
+        p.grad = torch.ones_like(p)
+    with pytest.raises(ValueError):
+        opt.step()

@@ -41,3 +41,72 @@ def test_eight_bit_checkpoint_resumed_in_32_bits(tmp_path, kind):
     # by a rounded constant (a rounding less)
     worst = abs(b.flat_p[:n].double().cpu().numpy() - p2) - dp
     assert worst.max() <= 0, worst.max()
+
+
+def _one_step(p, g, m, v, lr, t, got, master, rounding):
+    """got and master, if there is one, against the oracle's step (decay 0.01)."""
+    (p2, m2, v2), (dp, _, _, _) = O.step(p, g, m, v, lr, t, (0.9, 0.999), 1e-8, 0.01)
+    if master is not None:
+        assert (abs(master - p2) - dp).max() <= 0
+        p2, dp = master, 0.0
+    assert (abs(got - p2) - dp - rounding * (abs(p2) + dp)).max() <= 0
+    return m2, v2
+
+
+@pytest.mark.parametrize("dtype,half", [(torch.bfloat16, 2.0 ** -8), (torch.float16, 2.0 ** -11)])
+def test_weights_loaded_after_a_step(dtype, half):
+    """Weights loaded in place, their masters dropped: the next step starts from the loaded weights, and the state has masters again.  A master that
+    is assigned is the one that the step reads."""
+    from benerf_amd import optim
+    f64 = lambda t: t.detach().double().cpu().numpy().reshape(-1)      # noqa: E731
+    gen = torch.Generator().manual_seed(5)
+    rand = lambda *s: torch.randn(*s, generator=gen)      # noqa: E731
+    ps = [torch.nn.Parameter((rand(40, 33) + 3).to(dtype).cuda()), torch.nn.Parameter(rand(7).cuda()), torch.nn.Parameter((rand(129) + 3).to(dtype).cuda())]
+    opt = optim.FusedAdamW(ps, lr=1e-2, master=True)
+
+    def step():
+        for p in ps:
+            p.grad = (rand(*p.shape) * 0.1 + 0.05).to(p.dtype).cuda()
+        opt.step()
+    step()
+    with torch.no_grad():
+        for p in ps:
+            p.copy_((rand(*p.shape) - 5).to(p.dtype))
+    for p in (ps[0], ps[2]):
+        del opt.state[p]["master"]
+    for t in (2, 3):
+        before = [(f64(opt.state[p].get("master", p)), f64(opt.state[p]["exp_avg"]), f64(opt.state[p]["exp_avg_sq"])) for p in ps]
+        step()
+        for p, (x, m, v) in zip(ps, before):
+            master = opt.state[p]["master"] if p.dtype == dtype else None
+            _one_step(x, f64(p.grad), m, v, 1e-2, t, f64(p), None if master is None else f64(master), half if p.dtype == dtype else 0.0)
+    mine = torch.full((129,), 7.0, device="cuda")
+    opt.state[ps[2]]["master"] = mine
+    m, v = f64(opt.state[ps[2]]["exp_avg"]), f64(opt.state[ps[2]]["exp_avg_sq"])
+    step()
+    _one_step(f64(torch.full((129,), 7.0)), f64(ps[2].grad), m, v, 1e-2, 4, f64(ps[2]), f64(mine), half)
+
+
+def test_assigned_scales_are_read():
+    """The scale of every block doubled by assignment: the step reads moments twice as large, and writes its scales into the assigned tensors."""
+    from benerf_amd import optim
+    f64 = lambda t: t.detach().double().cpu().numpy().reshape(-1)      # noqa: E731
+    p = torch.nn.Parameter(torch.randn(700, generator=torch.Generator().manual_seed(1)).cuda())
+    opt = optim.FusedAdamW([p], lr=1e-2, state_bits=8)
+    for _ in range(2):
+        p.grad = torch.randn(700, generator=torch.Generator().manual_seed(2)).cuda()
+        opt.step()
+    st = opt.state[p]
+    for name in ("exp_avg_scale", "exp_avg_sq_scale"):
+        st[name] = st[name] * 2
+    m, u = (optim.decode_moment(st[name], st[name + "_scale"]) for name in ("exp_avg", "exp_avg_sq"))
+    before, m, v = f64(p), f64(m), f64(u) ** 2
+    held = st["exp_avg_scale"], st["exp_avg_sq_scale"]
+    kept = [x.clone() for x in held]
+    p.grad = torch.zeros(700, device="cuda")
+    opt.step()
+    (p2, m2, v2), (dp, _, _, _) = O.step(before, 0 * before, m, v, 1e-2, 3, (0.9, 0.999), 1e-8, 0.01)
+    assert (abs(f64(p) - p2) - dp).max() <= 0
+    # m shrinks by a tenth and u by 0.05 %: a block's scale stays, or halves where its largest value falls below a power of two
+    for x, y, name in zip(held, kept, ("exp_avg_scale", "exp_avg_sq_scale")):
+        assert opt.state[p][name] is x and bool(((x == y) | (x == y / 2)).all())
