@@ -219,9 +219,11 @@ class FlatAdam(torch.optim.Adam):
         return None
 
 
-def encode_moment(x):
+def encode_moment(x, root=False):
     """A float32 moment in 8 bits, to nearest: (float8_e4m3fn codes of x's shape, float32 scale of every 128 consecutive elements).  For
-    a checkpoint of 32-bit moments; the step itself rounds stochastically (include/benerf_hip.h, K9).  Encode the ROOT of exp_avg_sq."""
+    a checkpoint of 32-bit moments; the step itself rounds stochastically (include/benerf_hip.h, K9).  Encode the ROOT of exp_avg_sq, with
+    root=True: what is above 0 then becomes 2^-9 of its scale at least, as in the step - exp_avg has a scale of its own, and the next update must
+    not be divided by eps alone."""
     n = x.numel()
     pad = torch.zeros(-(-n // K.ADAMW_BLOCK) * K.ADAMW_BLOCK, dtype=torch.float32, device=x.device)
     pad[:n] = x.detach().reshape(-1)
@@ -229,7 +231,10 @@ def encode_moment(x):
     top = torch.where(rows.isfinite(), rows.abs(), 0.0).amax(1)
     exponent = (torch.frexp(top)[1] - 1).clamp_min(-100) - 7
     scale = ((exponent.to(torch.int32) + 127) << 23).view(torch.float32)
-    code = torch.where(rows.isfinite(), rows / scale[:, None], float("nan")).view(-1)[:n]
+    grid = rows / scale[:, None]
+    if root:
+        grid = torch.where(rows > 0, grid.clamp_min(2.0 ** -9), grid)
+    code = torch.where(rows.isfinite(), grid, float("nan")).view(-1)[:n]
     return code.to(K.CODE_TYPE).view(x.shape), scale
 
 
@@ -265,7 +270,7 @@ def convert_moments(state, bits):
         return {"exp_avg": decode_moment(state["exp_avg"], state["exp_avg_scale"]), "exp_avg_sq": decode_moment(state["exp_avg_sq"], state["exp_avg_sq_scale"]).square_()}
     out = {}
     out["exp_avg"], out["exp_avg_scale"] = encode_moment(state["exp_avg"].to(torch.float32))
-    out["exp_avg_sq"], out["exp_avg_sq_scale"] = encode_moment(state["exp_avg_sq"].to(torch.float32).sqrt())
+    out["exp_avg_sq"], out["exp_avg_sq_scale"] = encode_moment(state["exp_avg_sq"].to(torch.float32).sqrt(), root=True)
     return out
 
 

@@ -155,3 +155,31 @@ def test_dropped_and_assigned_moments_are_followed(plans):
         p.grad = torch.ones_like(p)
     with pytest.raises(ValueError):
         opt.step()
+
+
+def test_encoded_roots_above_zero_stay_above_zero():
+    """Of the second moment's root no value above 0 may become 0: with m on a scale of its own the next update would be divided by eps alone.  A
+    32-bit checkpoint in 8 bits takes the step that it takes in 32."""
+    from benerf_amd import optim
+    n = 300
+    u, m = torch.full((n,), 2.0 ** -18), torch.full((n,), 2.0 ** -18)
+    u[0], u[128], u[299], m[0], m[128], m[299] = 1.0, 1.5, 255.0, 0.01, -0.01, 0.01
+    u[5], m[5] = 0.0, 0.0
+    held = optim.convert_moments(dict(exp_avg=m, exp_avg_sq=u.square()), 8)
+    root = optim.decode_moment(held["exp_avg_sq"], held["exp_avg_sq_scale"])
+    least = 2.0 ** -9 * held["exp_avg_sq_scale"].repeat_interleave(128)[:n]
+    assert bool((root[u > 0] >= least[u > 0]).all()) and root[5] == 0
+    # values that nearest does not take to 0 are as they were, and moments with a sign may become 0
+    plain = optim.decode_moment(*optim.encode_moment(u))
+    assert torch.equal(root[plain > 0], plain[plain > 0]) and bool((plain[1:5] == 0).all())
+    assert bool((optim.decode_moment(*optim.encode_moment(torch.tensor([1.0, 2.0 ** -18, -2.0 ** -18])))[1:] == 0).all())
+    # the next step without a gradient, t = 1000: its size against the same in 32 bits
+    m8 = optim.decode_moment(held["exp_avg"], held["exp_avg_scale"])
+    bc2 = (1 - 0.999 ** 1000) ** 0.5
+    move8, move32 = (0.9 * x / (0.999 ** 0.5 * y / bc2 + 1e-8) for x, y in ((m8, root), (m, u)))
+    # a root is lifted, not lowered, here; m and u are powers of two or rounded to nearest by 2^-4 each
+    assert bool((move8.abs() <= 1.2 * move32.abs()).all())
+    # not finite: the elements of their own; an empty tensor
+    bad = optim.convert_moments(dict(exp_avg=torch.zeros(3), exp_avg_sq=torch.tensor([1.0, float("inf"), float("nan")])), 8)
+    assert bad["exp_avg_sq"].float()[1:].isnan().all() and optim.decode_moment(bad["exp_avg_sq"], bad["exp_avg_sq_scale"])[0] == 1.0
+    assert optim.convert_moments(dict(exp_avg=torch.zeros(0), exp_avg_sq=torch.zeros(0)), 8)["exp_avg_sq"].shape == (0,)

@@ -110,3 +110,22 @@ def test_assigned_scales_are_read():
     # m shrinks by a tenth and u by 0.05 %: a block's scale stays, or halves where its largest value falls below a power of two
     for x, y, name in zip(held, kept, ("exp_avg_scale", "exp_avg_sq_scale")):
         assert opt.state[p][name] is x and bool(((x == y) | (x == y / 2)).all())
+
+
+def test_a_32_bit_checkpoint_in_8_bits_moves_no_further():
+    """A block whose second moments span 2^36: roots far below the block's largest are lifted, not lost, so the first step in 8 bits is no longer than the
+    one in 32 (m and u to nearest, 2^-4 each)."""
+    from benerf_amd import optim
+    n, lr = 300, 1e-2
+    u, m = torch.full((n,), 2.0 ** -18), torch.full((n,), 2.0 ** -18)
+    u[0], u[128], u[299], m[0], m[128], m[299] = 1.0, 1.5, 255.0, 0.01, -0.01, 0.01
+    moved = []
+    for bits in (32, 8):
+        p = torch.nn.Parameter(torch.zeros(n, device="cuda"))
+        opt = optim.FusedAdamW([p], lr=lr, weight_decay=0.0, state_bits=bits)
+        state = {0: dict(step=torch.tensor(999.0), exp_avg=m.clone(), exp_avg_sq=u.square())}
+        opt.load_state_dict(dict(state=state, param_groups=opt.state_dict()["param_groups"]))
+        p.grad = torch.zeros_like(p)
+        opt.step()
+        moved.append(p.detach().abs())
+    assert bool((moved[1] <= 1.2 * moved[0]).all()) and bool((moved[0][1:128] > 0.5 * lr).all()) and float(opt.state[p]["step"]) == 1000.0
