@@ -299,7 +299,7 @@ class RenderPair(torch.autograd.Function):
         need_grad = any(ctx.needs_input_grad) and getattr(draws, "grad_enabled", True)      # the caller's grad mode: see RenderRays.forward
         if need_grad and K.is_split():
             K.range_guard(dev).poll()          # what the previous backward posted (see RenderRays.forward)
-        if net_c._key() != net_c.version or net_f._key() != net_f.version:
+        if net_c.stale() or net_f.stale():
             K.PackedMlp.pack_pair(net_c, net_f)        # one re-pack launch per optimiser step for both networks
         S, Ni = n_samples, n_importance
         Ne, Nr = pe.shape[0] * idx_e.shape[0], pr.shape[0] * idx_r.shape[0]

@@ -365,6 +365,11 @@ def params_changed():
     _param_generation += 1
 
 
+# Memory that a captured optimiser step writes at every replay, by address of the storage: no generation and no version counter moves then.
+# Where such an address comes to hold something else, that is packed too often, never too rarely.
+_replayed = set()
+
+
 class PackedMlp:
     """MFMA-shaped copy of one NeRF's weights; `pack()` after every optimiser step."""
 
@@ -402,9 +407,15 @@ class PackedMlp:
                                                     a.channels, _stream()), "mlp_pack_weights_pair")
         a.version, b.version = a._key(), b._key()
 
+    def stale(self):
+        """True if the weights may be others than those packed last.  torch updates bump ._version; updates through the raw Adam kernel /
+        in-place loads bump the generation; a captured step bumps neither at its replays, so what one may write is always packed again; and a
+        capture packs for its own replays."""
+        return (self._key() != self.version or torch.cuda.is_current_stream_capturing() or
+                bool(_replayed and any(t.untyped_storage().data_ptr() in _replayed for t in self.weights + self.biases)))
+
     def pack_if_stale(self):
-        # torch updates bump ._version; updates through the raw Adam kernel / in-place loads bump the generation
-        if self._key() != self.version:
+        if self.stale():
             self.pack()
 
 
@@ -962,7 +973,8 @@ def adamw_count(step, norm=None, guard_range=True, status=None):
 def adamw_step(plan, grads, lr, step, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.0, grad_scale=1.0, norm=None, seed=0, guard_range=True, status=None):
     """One AdamW step over the tensors of an AdamWPlan.  grads: GradList or a list (None: the tensor is left alone).  lr: a number, or
     one float32 on the device.  step: t of this step from 1, or one float32 on the device that holds it (adamw_count, grad_norm(counters=)
-    count) - needed in a captured step, whose numbers are frozen.  norm: what grad_norm returned - clips, and skips the step where it says
+    count) - needed in a captured step, whose numbers are frozen (a PackedMlp of these parameters is packed again before every forward pass from
+    then on; no replay between a forward pass and its backward).  norm: what grad_norm returned - clips, and skips the step where it says
     so; without a device counter t then counts applied steps.  seed: stochastic rounding of 8-bit moments.  guard_range, status: as in
     `adam_step`."""
     dev = plan.device
@@ -987,6 +999,8 @@ def adamw_step(plan, grads, lr, step, betas=(0.9, 0.999), eps=1e-8, weight_decay
     words = None if norm is None else _norm_words(norm, dev, "norm")
     guard = (plan.parts[0].guard if status is None else _guard_words(status, dev)) if guard_range else None
     stream = _stream()
+    if torch.cuda.is_current_stream_capturing():
+        _replayed.update(p.untyped_storage().data_ptr() for p in plan.params)
     for part, kind, ptrs in launches:
         part.used_on(stream)
         _lib.check(lib.benerf_adamw_step(part.host_at, part.dev_at, ptrs.buffer_info()[0], kind, cfg, words, guard, stream), "adamw_step")
