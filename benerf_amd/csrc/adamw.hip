@@ -540,11 +540,17 @@ int64_t count_chunks(const BenerfAdamwTensor* t, int n) {
     for (int k = 0; k < n; ++k) chunks += (t[k].n + CHUNK - 1) / CHUNK;
     return chunks;
 }
-int plan_shape(const BenerfAdamwTensor* t, int n, int param_type, int state_bits) {
+// the first tensor with elements says whether the list has masters: an empty one has no memory
+bool list_has_master(const BenerfAdamwTensor* t, int n, int state_bits) {
+    for (int k = 0; k < n && state_bits != 0; ++k)
+        if (t[k].n > 0) return t[k].master != nullptr;
+    return false;
+}
+int plan_shape(const BenerfAdamwTensor* t, int n, int param_type, int state_bits, bool master) {
     int64_t total = 0;
     for (int k = 0; k < n; ++k) total += t[k].n;
     const int width = type_bytes(param_type);
-    const int64_t bytes = total * (state_bits == 0 ? width : 2 * width + (state_bits == 8 ? 2 : 8) + (n > 0 && t[0].master ? 4 : 0));
+    const int64_t bytes = total * (state_bits == 0 ? width : 2 * width + (state_bits == 8 ? 2 : 8) + (master ? 4 : 0));
     return bytes > PAST_BYTES ? PAST : n <= PTRS_SMALL ? SHORT : MANY;
 }
 
@@ -645,7 +651,7 @@ extern "C" int benerf_adamw_plan_fill(const BenerfAdamwTensor* tensors_host, int
         benerf_set_error("adamw_plan_fill: %zu bytes, %zu needed", plan_bytes, need);
         return BENERF_EWORKSPACE;
     }
-    const bool master = tensors_host[0].master != nullptr;
+    const bool master = list_has_master(tensors_host, n_tensors, state_bits);
     BENERF_REQUIRE(!master || param_type != BENERF_F32, "adamw_plan_fill: a float32 parameter is its own master copy");
     for (int k = 0; k < n_tensors; ++k) {
         const BenerfAdamwTensor& t = tensors_host[k];
@@ -666,7 +672,7 @@ extern "C" int benerf_adamw_plan_fill(const BenerfAdamwTensor* tensors_host, int
     h->param_type = param_type;
     h->state_bits = state_bits;
     h->has_master = master;
-    h->shape = plan_shape(tensors_host, n_tensors, param_type, state_bits);
+    h->shape = plan_shape(tensors_host, n_tensors, param_type, state_bits, master);
     h->n_chunks = count_chunks(tensors_host, n_tensors);
     h->chunks_at = (int64_t)(HEAD_BYTES + sizeof(Entry) * (size_t)n_tensors);
     h->bytes = (int64_t)need;

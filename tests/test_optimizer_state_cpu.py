@@ -1,4 +1,6 @@
 """CPU: what becomes of optimiser state outside the kernels - checkpoints of one form read by the other - with the real host code on host tensors."""
+import ctypes
+import os
 from types import SimpleNamespace
 
 import pytest
@@ -183,3 +185,31 @@ def test_encoded_roots_above_zero_stay_above_zero():
     bad = optim.convert_moments(dict(exp_avg=torch.zeros(3), exp_avg_sq=torch.tensor([1.0, float("inf"), float("nan")])), 8)
     assert bad["exp_avg_sq"].float()[1:].isnan().all() and optim.decode_moment(bad["exp_avg_sq"], bad["exp_avg_sq_scale"])[0] == 1.0
     assert optim.convert_moments(dict(exp_avg=torch.zeros(0), exp_avg_sq=torch.zeros(0)), 8)["exp_avg_sq"].shape == (0,)
+
+
+def test_plans_whose_first_tensor_is_empty():
+    """An empty tensor has no memory, so neither masters nor anything else is read off it: wherever it stands, a list with masters is laid out, and
+    the others must all have theirs or none."""
+    from benerf_amd import _lib, build
+    if not os.path.exists(_lib.LIB_PATH):
+        build.build()
+    lib = _lib.load()
+
+    def fill(*rows, kind=1):
+        table = (_lib.AdamwTensor * len(rows))(*[_lib.AdamwTensor(**r) for r in rows])
+        size = lib.benerf_adamw_plan_bytes(table, len(rows))
+        buf = ctypes.create_string_buffer(size)
+        return lib.benerf_adamw_plan_fill(table, len(rows), kind, 32, buf, size), bytes(buf)[:48]
+    none = dict(n=0)
+    full = dict(param=0x1000, exp_avg=0x2000, exp_avg_sq=0x3000, n=5)
+    kept = dict(full, master=0x4000)
+    heads = [fill(*rows) for rows in ((kept, none), (none, kept), (none, none, kept, none), (kept, kept))]
+    assert [rc for rc, _ in heads] == [0, 0, 0, 0]
+    assert heads[0][1] == heads[1][1]                                   # type, bits, masters and shape are those of the same list in another order
+    assert fill(none, full)[0] == 0 and fill(none)[0] == 0 and fill(none, none)[0] == 0
+    for bad in ((none, kept, full), (none, full, kept), (full, none, kept)):
+        assert fill(*bad)[0] == -1 and b"master copies" in lib.benerf_last_error()
+    assert fill(none, kept, kind=0)[0] == -1 and b"its own master" in lib.benerf_last_error()
+    # past the caches from 320 MB on: 13 M bfloat16 with masters (2 + 2 + 8 + 4 bytes) and 30 M are on either side, an empty first tensor or not
+    for n in (13 << 20, 30 << 20):
+        assert fill(dict(kept, n=n), none)[1] == fill(none, dict(kept, n=n))[1]

@@ -205,3 +205,25 @@ def test_a_captured_pack_is_part_of_its_graph():
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(packed.packed.view(torch.int32), _fresh_pack(net))
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("order", [(0, 5), (5, 0), (0, 0, 700, 0)])
+def test_empty_parameters_with_masters(order, bits):
+    from benerf_amd import optim
+    f64 = lambda t: t.detach().double().cpu().numpy().reshape(-1)      # noqa: E731
+    gen = torch.Generator().manual_seed(7)
+    ps = [torch.nn.Parameter((torch.randn(n, generator=gen) + 3).to(torch.bfloat16).cuda()) for n in order]
+    start = [f64(p) for p in ps]
+    opt = optim.FusedAdamW(ps, lr=1e-2, master=True, max_norm=10.0, state_bits=bits)
+    for p in ps:
+        p.grad = torch.ones_like(p)
+    opt.step()
+    norm = sum(order) ** 0.5
+    assert abs(float(opt.grad_norm[0]) - norm) <= 2 * O.HALF * norm
+    scale = min(1.0, 10.0 / (norm + 1e-6))
+    for p, x in zip(ps, start):
+        if x.size:
+            (p2, _, _), (dp, _, _, _) = O.step(x, 0 * x + 1, 0 * x, 0 * x, 1e-2, 1, (0.9, 0.999), 1e-8, 0.01, scale)
+            master = f64(opt.state[p]["master"])
+            assert (abs(master - p2) - dp).max() <= 0 and (abs(f64(p) - master) - 2.0 ** -8 * abs(master)).max() <= 0
