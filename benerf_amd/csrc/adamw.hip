@@ -335,7 +335,8 @@ struct Four8 {
         }
         uint32_t top = block_max(pack_tops(__float_as_uint(fmaxf(fmaxf(fabsf(m[0]), fabsf(m[1])), fmaxf(fabsf(m[2]), fabsf(m[3])))), top_bits(root)));
         // The instruction takes denormal numbers for 0: their roots (below 2^-63) count where nothing else in the block does, or with an eps
-        // that they are not lost in.
+        // that they are not lost in.  The maximum found again is that of the finite ones, so the next branch is not taken behind this one: inf and NaN
+        // of any payload are left to the conversion, which makes them NaN (nine patterns, eight draws each).
         if (h.eps < 1e-11f || __any((top & 0xffffu) == 0u)) {
             for (int j = 0; j < 4; ++j) root[j] = sqrtf(v[j]);
             top = block_max(pack_tops(finite_top(m), finite_top(root)));

@@ -1,4 +1,5 @@
 """GPU: optimiser state between forms and owners - checkpoints of one networks' optimiser resumed with another."""
+import numpy as np
 import pytest
 import torch
 
@@ -43,6 +44,10 @@ def test_eight_bit_checkpoint_resumed_in_32_bits(tmp_path, kind):
     assert worst.max() <= 0, worst.max()
 
 
+def f64(t):
+    return t.detach().double().cpu().numpy().reshape(-1)
+
+
 def _one_step(p, g, m, v, lr, t, got, master, rounding):
     """got and master, if there is one, against the oracle's step (decay 0.01)."""
     (p2, m2, v2), (dp, _, _, _) = O.step(p, g, m, v, lr, t, (0.9, 0.999), 1e-8, 0.01)
@@ -58,7 +63,6 @@ def test_weights_loaded_after_a_step(dtype, half):
     """Weights loaded in place, their masters dropped: the next step starts from the loaded weights, and the state has masters again.  A master that
     is assigned is the one that the step reads."""
     from benerf_amd import optim
-    f64 = lambda t: t.detach().double().cpu().numpy().reshape(-1)      # noqa: E731
     gen = torch.Generator().manual_seed(5)
     rand = lambda *s: torch.randn(*s, generator=gen)      # noqa: E731
     ps = [torch.nn.Parameter((rand(40, 33) + 3).to(dtype).cuda()), torch.nn.Parameter(rand(7).cuda()), torch.nn.Parameter((rand(129) + 3).to(dtype).cuda())]
@@ -90,7 +94,6 @@ def test_weights_loaded_after_a_step(dtype, half):
 def test_assigned_scales_are_read():
     """The scale of every block doubled by assignment: the step reads moments twice as large, and writes its scales into the assigned tensors."""
     from benerf_amd import optim
-    f64 = lambda t: t.detach().double().cpu().numpy().reshape(-1)      # noqa: E731
     p = torch.nn.Parameter(torch.randn(700, generator=torch.Generator().manual_seed(1)).cuda())
     opt = optim.FusedAdamW([p], lr=1e-2, state_bits=8)
     for _ in range(2):
@@ -211,7 +214,6 @@ def test_a_captured_pack_is_part_of_its_graph():
 @pytest.mark.parametrize("order", [(0, 5), (5, 0), (0, 0, 700, 0)])
 def test_empty_parameters_with_masters(order, bits):
     from benerf_amd import optim
-    f64 = lambda t: t.detach().double().cpu().numpy().reshape(-1)      # noqa: E731
     gen = torch.Generator().manual_seed(7)
     ps = [torch.nn.Parameter((torch.randn(n, generator=gen) + 3).to(torch.bfloat16).cuda()) for n in order]
     start = [f64(p) for p in ps]
@@ -227,3 +229,42 @@ def test_empty_parameters_with_masters(order, bits):
             (p2, _, _), (dp, _, _, _) = O.step(x, 0 * x + 1, 0 * x, 0 * x, 1e-2, 1, (0.9, 0.999), 1e-8, 0.01, scale)
             master = f64(opt.state[p]["master"])
             assert (abs(master - p2) - dp).max() <= 0 and (abs(f64(p) - master) - 2.0 ** -8 * abs(master)).max() <= 0
+
+
+PATTERNS = (0x7fc00000, 0xffc00000, 0x7fffffff, 0xffffffff, 0x7f800001, 0xff800001, 0x7fbfffff, 0x7f800000, 0xff800000)
+
+
+@pytest.mark.parametrize("eps", [1e-8, 1e-15])
+@pytest.mark.parametrize("n", [1, 100, 128, 129, 300, 640])
+def test_non_finite_gradients_in_8_bits_beside_empty_blocks(n, eps):
+    """inf and NaN of every kind in one element of a tensor whose other block of the wavefront is empty, zero or ordinary, over many draws: both codes of
+    that element are NaN and stay it, every other element takes the step of the formula, block scales included.  (Bit for bit the others need not be what
+    they are without: the root of a wavefront with an empty block is rounded correctly, others to 1 ulp.)"""
+    from benerf_amd import kernels as K, optim
+    gen = torch.Generator().manual_seed(n)
+    clean = torch.randn(n, generator=gen)
+    clean[128:256] = 0.0                                               # a block of zeros, if there is one
+    for k, word in enumerate(PATTERNS):
+        at = (n - 1, 0, n // 2)[k % 3]
+        others = np.arange(n) != at
+        p = torch.zeros(n, device="cuda")
+        moments = optim.zero_moments([p], 8)
+        plan = K.AdamWPlan([p], **moments)
+        g = clean.clone()
+        g.view(torch.int32)[at] = int(np.uint32(word).astype(np.int32))
+        g = g.cuda()
+        x, m, u = (np.where(others, np.nan_to_num(y), 0.0) for y in (f64(p), np.zeros(n), np.zeros(n)))
+        for t in range(1, 9):
+            K.adamw_step(plan, [g], 1e-2, t, eps=eps, weight_decay=0.01, seed=k)
+            (p2, m2, v2), (dp, dm, dv, du) = O.step(x, np.where(others, f64(clean), 0.0), m, u * u, 1e-2, t, (0.9, 0.999), eps, 0.01)
+            assert np.isnan(f64(p)[at]) and np.all(np.abs(f64(p) - p2)[others] <= dp[others]), (hex(word), t)
+            got = []
+            for name, y, dy, r, keep in (("exp_avg", m2, dm, O.draws(n, 0, t, k)[0], False), ("exp_avg_sq", np.sqrt(v2), du, O.draws(n, 0, t, k)[1], True)):
+                code, scale = f64(moments[name][0].float()), f64(moments[name + "_scale"][0])
+                assert np.isnan(code[at]), (hex(word), t, name, code[at])
+                value = code * np.repeat(scale, 128)[:n]
+                low, high = O.coded_range(y, dy, r, keep)
+                assert np.all(((low <= np.abs(value)) & (np.abs(value) <= high))[others]), (hex(word), t, name)
+                assert np.all((scale >= O.scale_of(np.maximum(np.abs(y) - dy, 0))) & (scale <= O.scale_of(np.abs(y) + dy))), (hex(word), t, name)
+                got.append(value)
+            x, m, u = (np.where(others, y, 0.0) for y in (f64(p), *got))
