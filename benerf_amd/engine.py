@@ -463,6 +463,10 @@ class TrainStep:
     is not finite, leaves parameters and Adam moments untouched on every rank and is counted on the device; Adam's bias
     correction counts APPLIED steps only (t = iteration - skipped steps, like torch's GradScaler), the LR schedule follows the
     iteration count like the reference's (train.py:355-394).
+
+    Networks under AdamW with args.benerf_max_grad_norm: where the norm of their gradients is not finite, their part of the step is skipped and
+    counted; the trajectory, which steps before those gradients are complete, and the tone-mappers are not gated by it.  step() raises when nothing
+    but such steps lie between two of its looks at the counters, MAX_SKIPPED_IN_A_ROW or more, check_range() at any.
     """
     MAX_SKIPPED_IN_A_ROW = 3     # consecutive range-guard skips after which step() raises (checked without synchronising)
     GUARD_POST_EVERY = 8         # steps between two copies of the guard's counters to the host
@@ -598,6 +602,8 @@ class TrainStep:
         self.net_c.packed.pack()
         self.net_f.packed.pack()
         self.last_losses = None
+        self._norm_mirror, self._norm_told, self._norm_seen = None, 0, (0, 0)
+        self._norm_from_here()
 
     # -- schedule (train.py:355-394) ------------------------------------------------------------
     def _lr(self, lr0, decay):
@@ -672,6 +678,7 @@ class TrainStep:
         self.global_step = int(global_step)
         skipped = 0 if applied is None else max(self.global_step - applied, 0)
         self.guard.words[_lib.ST_SKIPPED_TOTAL:_lib.ST_SKIPPED_TOTAL + 1].fill_(skipped)
+        self._norm_from_here()
         self._prefetched = None
         self.net_c.packed.pack()
         self.net_f.packed.pack()
@@ -689,8 +696,58 @@ class TrainStep:
 
     def check_range(self, reset=True):
         """Synchronises.  Raises kernels.BenerfRangeError if a step since the last reset left the f16 range of the split mode
-        (those steps were skipped on every rank: parameters and Adam moments untouched)."""
+        (those steps were skipped on every rank: parameters and Adam moments untouched), or if the norm of the networks' gradients was not finite
+        in one (the networks' part of it was skipped)."""
         self.guard.check(reset)
+        if self.max_grad_norm is not None:
+            self._norm_posted = None            # older than this look
+            skips = self._norm_skips(self.net_norm, self.guard.words[_lib.ST_SKIPPED_TOTAL])
+            told = self._norm_told
+            if reset:
+                self._norm_told = skips
+            if skips > told:
+                self._raise_norm(skips - told)
+
+    # -- steps that the norm of the networks' gradients skips: seen like the guard's, from copies that land in pinned memory -------------
+    @staticmethod
+    def _norm_skips(words, guard_total):
+        """Steps skipped by the norm alone: its own count holds those of the range guard too."""
+        return int(words[3]) - int(guard_total)
+
+    def _norm_from_here(self):
+        """Begins counting anew (synchronises): nothing skipped before this is told."""
+        self._norm_posted, self._norm_run = None, 0
+        if self.max_grad_norm is not None:
+            self._norm_told = self._norm_skips(self.net_norm, self.guard.words[_lib.ST_SKIPPED_TOTAL])
+            self._norm_seen = (self.global_step, self._norm_told)
+
+    def _post_norm(self, done):
+        if self._norm_mirror is None:
+            self._norm_mirror = (torch.zeros(4, dtype=torch.float32, device="cpu").pin_memory(), torch.zeros(1, dtype=torch.int32, device="cpu").pin_memory())
+            self._norm_event = torch.cuda.Event()
+        for host, words in zip(self._norm_mirror, (self.net_norm, self.guard.words[_lib.ST_SKIPPED_TOTAL:_lib.ST_SKIPPED_TOTAL + 1])):
+            host.copy_(words, non_blocking=True)
+        self._norm_event.record()
+        self._norm_posted = done
+
+    def _poll_norm(self):
+        """Non-blocking.  Raises BenerfRangeError when all steps between copies that have landed were skipped by the norm, MAX_SKIPPED_IN_A_ROW of
+        them or more."""
+        if self._norm_posted is None or not self._norm_event.query():
+            return
+        now, self._norm_posted = (self._norm_posted, self._norm_skips(self._norm_mirror[0], self._norm_mirror[1])), None
+        steps, skips = now[0] - self._norm_seen[0], now[1] - self._norm_seen[1]
+        self._norm_seen = now
+        self._norm_run = self._norm_run + steps if skips >= steps else 0
+        if self._norm_run >= self.MAX_SKIPPED_IN_A_ROW:
+            run, self._norm_run = self._norm_run, 0             # told once
+            self._norm_told = now[1]
+            self._raise_norm(run)
+
+    @staticmethod
+    def _raise_norm(n):
+        raise _lib.BenerfRangeError("the norm of the networks' gradients was not finite in %d training steps: their networks were left as they were on the "
+                                    "device, while trajectory and tone-mappers, which the norm does not gate, stepped" % n)
 
     def shard(self, idx_evt, idx_rgb):
         """This rank's contiguous slices of the global event / blur pixel-index vectors."""
@@ -769,6 +826,7 @@ class TrainStep:
         # range guard: a run whose steps keep being skipped on the device must not go on silently - looks at the last copy
         # of the counters that has landed in pinned host memory (no synchronisation)
         self.guard.poll(max_consecutive=self.MAX_SKIPPED_IN_A_ROW)
+        self._poll_norm()
         st = self.guard.words
         P = cfg.num_interpolated_pose
         S, Ni = cfg.N_samples, cfg.N_importance
@@ -1033,6 +1091,8 @@ class TrainStep:
             adam(lo, cnt, self._lr(lr0, dr))
         if self.global_step % self.GUARD_POST_EVERY == 0:
             self.guard.post()
+            if cfg.optimize_nerf and self.max_grad_norm is not None:
+                self._post_norm(self.global_step + 1)
         K.PackedMlp.pack_pair(self.net_c.packed, self.net_f.packed)
         self.global_step += 1
         self.last_losses = losses

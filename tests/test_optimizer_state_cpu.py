@@ -36,11 +36,11 @@ class _Step:
             self.net_moments = optim.zero_moments(nets, 8) if net_bits == 8 else \
                 {"exp_avg": [self.flat_m[:300], self.flat_m[300:305]], "exp_avg_sq": [self.flat_v[:300], self.flat_v[300:305]]}
         self.cfg = SimpleNamespace(lrate=LR, decay_rate=0.1, pose_lrate=LR, decay_rate_pose=0.1, transform_lrate=LR, decay_rate_transform=0.1, lrate_decay=10)
-        self.crf_groups, self.global_step = [], 0
+        self.crf_groups, self.global_step, self.max_grad_norm = [], 0, None
         self.guard = SimpleNamespace(words=torch.zeros(16, dtype=torch.int32))
         packed = SimpleNamespace(packed=SimpleNamespace(pack=lambda: None))
         self.net_c = self.net_f = packed
-        for name in ("_lr", "_flat_slice", "_network_places", "_trained_optimizers", "import_optimizer_state"):
+        for name in ("_lr", "_flat_slice", "_network_places", "_trained_optimizers", "_norm_from_here", "import_optimizer_state"):
             setattr(self, name, getattr(engine.TrainStep, name).__get__(self))
 
     def moments(self, k):

@@ -268,3 +268,62 @@ def test_non_finite_gradients_in_8_bits_beside_empty_blocks(n, eps):
                 assert np.all((scale >= O.scale_of(np.maximum(np.abs(y) - dy, 0))) & (scale <= O.scale_of(np.abs(y) + dy))), (hex(word), t, name)
                 got.append(value)
             x, m, u = (np.where(others, y, 0.0) for y in (f64(p), *got))
+
+
+@pytest.mark.parametrize("every", [1, 4])
+def test_steps_skipped_by_the_norm_are_reported(every):
+    """A norm that is not finite step after step: the networks stay, and step() raises from the copies that it keeps of the counters, without a
+    synchronisation of its own; a single skipped step passes; steps that the range guard skips are not counted here; check_range() sees both."""
+    from benerf_amd import _lib, engine, kernels as K
+    args, cam, HW, accu, img = _setting(benerf_optimizer="adamw", benerf_max_grad_norm=1.0)
+    _, g = _graph(args, seed=3)
+    step = engine.TrainStep(g, args, cam, cam, torch.device(DEV), seed=21)
+    step.GUARD_POST_EVERY = every
+    real = K.grad_norm
+
+    def poisoned(grads, *a, **kw):
+        step.flat_g[5] = float("nan")
+        return real(grads, *a, **kw)
+
+    def run(n, bad):
+        K.grad_norm = poisoned if bad else real
+        try:
+            for _ in range(n):
+                _run(step, HW, accu, img, step.global_step, step.global_step + 1)
+                torch.cuda.synchronize()
+        finally:
+            K.grad_norm = real
+    run(3, False)
+    step.check_range()
+    run(2, True)
+    run(2 * every, False)                     # a short run of skips is no error while training
+    with pytest.raises(_lib.BenerfRangeError, match="norm"):
+        step.check_range()
+    step.check_range()                        # told once
+    before = step.flat_p[:2 * step.n_net].clone()
+    knots = step.knots.clone()
+    at = step.global_step
+    with pytest.raises(_lib.BenerfRangeError, match="norm"):
+        run(3 * max(every, 3), True)
+    assert step.global_step - at <= 2 * every + 3 and torch.equal(step.flat_p[:2 * step.n_net], before)
+    # the trajectory, whose gradients were finite, went on; nothing of it is gated by the networks' norm
+    assert bool(step.flat_p[2 * step.n_net:].isfinite().all()) and not torch.equal(step.knots, knots)
+    run(2 * every, False)                     # told once, and training goes on
+    assert not torch.equal(step.flat_p[:2 * step.n_net], before)
+    # the guard's own skips are its own: [SKIP] set for every step by a poisoned verdict
+    step.check_range()
+    total = float(step.net_norm[3])
+    gate = step.guard.gate
+
+    def closed(flag=None, phase=1):
+        step.guard.words[_lib.ST_ACT] = 0x7f800000
+        gate(flag, phase)
+    step.guard.gate = closed
+    with pytest.raises(_lib.BenerfRangeError, match="f16 range"):
+        run(3 * max(every, 3), False)
+    step.guard.gate = gate
+    assert float(step.net_norm[3]) >= total + 3
+    with pytest.raises(_lib.BenerfRangeError, match="f16 range"):
+        step.check_range()
+    step.check_range()
+    run(2 * every, False)
