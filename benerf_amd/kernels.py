@@ -724,7 +724,18 @@ def _list_tensor(t, name, device, dtypes, numel=None):
     return t.detach()
 
 
-_captured = {}                      # plans' tables that captured launches read at every replay: never freed
+_captured = {}                      # plans' tables that captured launches read at every replay: kept until release_captured()
+
+
+def release_captured():
+    """Lets go of the plans' tables (80 bytes for every 512 elements) that are kept because a captured launch reads them.  For programs that capture again and
+    again: call it when graphs are gone.  A graph whose AdamWPlan, GradList or FusedAdamW is alive goes on as before, and as long as that is; one that
+    has outlived it must not be replayed any more.  Synchronises; not inside a captured region."""
+    if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
+        raise _lib.BenerfHipError("release_captured: not inside a captured region")
+    for device in {t.device for t in _captured.values()}:
+        torch.cuda.synchronize(device)
+    _captured.clear()
 
 
 _address, _numel, _dtype, _detach = torch.Tensor.data_ptr, torch.Tensor.numel, operator.attrgetter("dtype"), torch.Tensor.detach
@@ -841,7 +852,8 @@ class AdamWPlan:
     ceil(n / 128) elements each (moments in 8 bits; exp_avg_sq then holds the codes of the ROOT of the second moment).  master: None, or
     float32 copies of the parameters that are bfloat16 / float16 (None at the float32 ones): the step reads and updates those and rounds
     them into the parameters.  All tensors are updated where they are; the plan keeps them alive and must be made again when a parameter
-    moves.  Making one copies a table to the device and waits for it: not inside a captured region.  Calls for one plan are ordered by
+    moves.  Making one copies a table to the device and waits for it: not inside a captured region.  A table that a captured launch reads outlives its
+    plan, until release_captured().  Calls for one plan are ordered by
     the caller, like any writes to its tensors: two streams must not step it at once."""
 
     def __init__(self, params, exp_avg, exp_avg_sq, exp_avg_scale=None, exp_avg_sq_scale=None, master=None):

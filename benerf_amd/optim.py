@@ -348,7 +348,8 @@ class FusedAdamW(torch.optim.AdamW):
       capturable  counters live on the device, a step can be captured (make one step before, outside; learning rates that change need
                   `lr` as a float32 tensor on the device).  With max_norm they live there too.  A captured step goes on with the state,
                   the counters and the set of gradients of its capture: load_state_dict, or a step outside with other gradients
-                  missing, needs a new capture.  Networks whose weights it changes are packed again at every forward pass, and must not be
+                  missing, needs a new capture; a program that makes many of them with new optimisers calls kernels.release_captured()
+                  between them.  Networks whose weights it changes are packed again at every forward pass, and must not be
                   replayed over between a forward pass and its backward.
       guard_range skip the step where the MLP's range guard says so, like FlatAdam.
     state[p]["step"] is ONE tensor for all parameters of a group that have made the same steps (state_dict gives each its own).

@@ -327,3 +327,49 @@ def test_steps_skipped_by_the_norm_are_reported(every):
         step.check_range()
     step.check_range()
     run(2 * every, False)
+
+
+def test_tables_of_captured_plans_can_be_released():
+    """Captures with plans that are let go: their tables stay, and go when they are released; a graph whose plan lives replays on."""
+    import gc
+    from benerf_amd import _lib, kernels as K, optim
+
+    def capture():
+        p, g = [torch.ones(100000, device="cuda")], [torch.ones(100000, device="cuda")]
+        plan = K.AdamWPlan(p, **optim.zero_moments(p, 32))
+        grads, step = K.GradList(g, plan), torch.zeros((), device="cuda")
+        K.grad_norm(grads, counters=[step])
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            K.grad_norm(grads, counters=[step])
+            K.adamw_step(plan, grads, 1e-2, step, weight_decay=0.0)
+        return p, plan, grads, step, graph
+    K.release_captured()
+    kept = capture()
+    assert len(K._captured) == 1
+    for _ in range(4):
+        capture()
+    gc.collect()
+    tables = 80 * 196 * 4                       # 196 pieces of 512 elements each
+    held = torch.cuda.memory_allocated()
+    assert len(K._captured) == 5
+    K.release_captured()
+    gc.collect()
+    assert not K._captured and held - torch.cuda.memory_allocated() >= tables
+    filled = [torch.full((16 << 10,), 255, dtype=torch.uint8, device="cuda") for _ in range(64)]
+    p, plan, grads, step, graph = kept
+    for t in (2, 3, 4):
+        graph.replay()
+        torch.cuda.synchronize()
+        # gradients of ones: m / (1 - b1^t) and v / (1 - b2^t) are 1 after steps 1 .. t, and the first here is t = 2 on moments of zero
+        assert float(step) == t and bool((p[0] == p[0][0]).all())
+    assert 1.0 - 3 * 1e-2 * 1.1 <= float(p[0][0]) < 1.0 and len(filled) == 64
+    refused = []
+    side = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(side):
+        torch.zeros(1, device="cuda")
+        try:
+            K.release_captured()
+        except _lib.BenerfHipError as e:
+            refused.append(str(e))
+    assert refused
