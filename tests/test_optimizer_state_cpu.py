@@ -213,3 +213,26 @@ def test_plans_whose_first_tensor_is_empty():
     # past the caches from 320 MB on: 13 M bfloat16 with masters (2 + 2 + 8 + 4 bytes) and 30 M are on either side, an empty first tensor or not
     for n in (13 << 20, 30 << 20):
         assert fill(dict(kept, n=n), none)[1] == fill(none, dict(kept, n=n))[1]
+
+
+def test_what_a_caller_keeps_in_the_state_is_left_alone(plans):
+    """Entries of the caller's own come and go without a new plan; together with a replaced or dropped tensor they hide nothing."""
+    from benerf_amd import optim
+    params = [torch.nn.Parameter(torch.zeros(5, dtype=torch.bfloat16)), torch.nn.Parameter(torch.zeros(3))]
+    opt = optim.FusedAdamW(params, master=True)
+    _steps(opt, params)
+    for p in params:
+        for value in (1, 2):
+            opt.state[p]["mine"] = value
+            _steps(opt, params)
+        del opt.state[p]["mine"]
+        _steps(opt, params)
+    assert len(plans) == 1 and float(opt.state[params[0]]["step"]) == 7.0
+    del opt.state[params[0]]["master"]
+    opt.state[params[0]]["mine"] = 1            # as many entries as before
+    _steps(opt, params)
+    assert len(plans) == 2 and "master" in opt.state[params[0]]
+    last = opt.state[params[1]]
+    del last["step"]                            # the last entry of all, or not
+    _steps(opt, params)
+    assert len(plans) == 3 and float(last["step"]) == 1.0 and float(opt.state[params[0]]["step"]) == 9.0
