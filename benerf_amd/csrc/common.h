@@ -27,6 +27,15 @@ void benerf_set_error(const char* fmt, ...);
 
 static inline hipStream_t as_stream(benerf_stream_t s) { return reinterpret_cast<hipStream_t>(s); }
 
+// Clears a few words on the stream.  A kernel, not hipMemsetAsync: a caller may capture the launch, and a captured memset has given wrong results
+// on replays after the first.
+static __global__ void benerf_clear_kernel(uint32_t* words, int n) {
+    for (int k = threadIdx.x; k < n; k += blockDim.x) words[k] = 0u;
+}
+static inline void benerf_clear_words(void* words, int n, hipStream_t stream) {
+    hipLaunchKernelGGL(benerf_clear_kernel, dim3(1), dim3(64), 0, stream, static_cast<uint32_t*>(words), n);
+}
+
 // hipFuncSetAttribute(MaxDynamicSharedMemorySize) applies to the function ON THE CURRENT DEVICE: set once per (call site,
 // device), not once per process - a process that launches on cuda:1 after cuda:0 needs it there too.
 struct BenerfLdsAttr { unsigned long long done; };

@@ -910,10 +910,7 @@ int benerf_mlp_dx_split22_launch(const BenerfMlpParams* params, const float* pac
     BENERF_REQUIRE(tiles < (1ll << 31), "mlp_bwd: too many points");
     if (!d_raw_absmax) {    // nobody computed max |d_raw| for us: one pass over d_raw into the info word
         float* info = dacts + mlp::sdact_info(mlp::m_pad(M));
-        if (hipMemsetAsync(info, 0, mlp::SD_COUNT * sizeof(float), stream) != hipSuccess) {
-            benerf_set_error("mlp_bwd: memset failed");
-            return BENERF_EHIP;
-        }
+        benerf_clear_words(info, mlp::SD_COUNT, stream);
         hipLaunchKernelGGL(grad_absmax22_kernel, dim3(256), dim3(256), 0, stream, d_raw, M * (channels + 1), info + mlp::SD_DRAW);
     }
     dim3 grid((unsigned)tiles), block(BNT);

@@ -378,10 +378,7 @@ extern "C" int benerf_mlp_fwd(const BenerfMlpParams* params, const float* packed
     const uint32_t* gate = nullptr;
     if (precision != BENERF_MLP_F32) {
         if (precision == BENERF_MLP_AUTO) {   // per-call maximum in status[3]; the f32 launch below runs only if it left the range
-            if (hipMemsetAsync(status + 3, 0, sizeof(uint32_t), as_stream(stream)) != hipSuccess) {
-                benerf_set_error("mlp_fwd: memset failed");
-                return BENERF_EHIP;
-            }
+            benerf_clear_words(status + 3, 1, as_stream(stream));
             gate = status + 3;
         }
         // BENERF_MLP_SPLIT_F16BWD (training and inference alike) runs the unfused layer sequence: its backward wants `feature`

@@ -373,3 +373,83 @@ def test_tables_of_captured_plans_can_be_released():
         except _lib.BenerfHipError as e:
             refused.append(str(e))
     assert refused
+
+
+@pytest.mark.parametrize("precision", ["split", "split_f16bwd", "f32"])
+def test_a_network_trained_inside_a_graph(precision):
+    """Forward, backward and step of a network on its points in one graph, replayed several times beside eager work on another network: every replay's loss
+    and weights are those of an eager twin."""
+    from benerf_amd import kernels as K, optim
+    K.set_mlp_precision(precision)
+    try:
+        gen = torch.Generator().manual_seed(6)
+        batches = [(torch.rand(40, 3, 3, generator=gen).to(DEV), torch.nn.functional.normalize(torch.randn(40, 3, generator=gen), dim=1).to(DEV)) for _ in range(8)]
+
+        def build():
+            net = _network(5)
+            return net, optim.FusedAdamW(net.parameters(), lr=1e-3, capturable=True, max_norm=1.0)
+
+        def once(net, opt, pts, dirs):
+            opt.zero_grad(set_to_none=True)
+            loss = (net(0, pts, dirs, None) ** 2).mean()
+            loss.backward()
+            opt.step()
+            return loss.detach()
+        (na, a), (nb, b) = build(), build()
+        other = _network(7)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            for k in range(2):
+                once(na, a, *batches[k])
+                once(nb, b, *batches[k])
+        torch.cuda.current_stream().wait_stream(side)
+        held = [x.clone() for x in batches[0]]
+        graph = torch.cuda.CUDAGraph()
+        a.zero_grad(set_to_none=True)
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph):
+            la = once(na, a, *held)
+        for k in range(2, 8):
+            for x, y in zip(held, batches[k]):
+                x.copy_(y)
+            graph.replay()
+            torch.cuda.synchronize()
+            lb = once(nb, b, *batches[k])
+            assert float(la) == float(lb), k
+            for p, q in zip(na.parameters(), nb.parameters()):
+                assert torch.equal(p, q), k
+            with torch.no_grad():
+                out = other(0, *batches[k - 1], None)          # an inference launch, and a render of the trained network
+                assert torch.equal(na(0, *batches[k - 1], None), nb(0, *batches[k - 1], None)) and bool(out.isfinite().all())
+            torch.cuda.synchronize()
+        assert float(a.state[next(na.parameters())]["step"]) == 8.0 and float(a.grad_norm[3]) == 0.0
+    finally:
+        K.set_mlp_precision("split")
+
+
+def test_a_captured_inference_launch():
+    """An inference launch of a network, captured and replayed over changing weights and points: its own overflow word starts from zero every time."""
+    net = _network(8)
+    twin = _network(8)
+    gen = torch.Generator().manual_seed(9)
+    batches = [(torch.rand(40, 3, 3, generator=gen).to(DEV), torch.nn.functional.normalize(torch.randn(40, 3, generator=gen), dim=1).to(DEV)) for _ in range(6)]
+    held = [x.clone() for x in batches[0]]
+    with torch.no_grad():
+        net(0, *held, None)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = net(0, *held, None)
+        for k in range(6):
+            # every second time the first layer overflows float16, so that the launch falls back to float32; the next one must not
+            with torch.no_grad():
+                for n in (net, twin):
+                    for li, layer in enumerate(n.pts_linears):
+                        layer.weight.mul_((300.0 if li == 0 else 3.0) if k % 2 else (1 / 300.0 if li == 0 else 1 / 3.0) if k else 1.0)
+            for x, y in zip(held, batches[k]):
+                x.copy_(y)
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, twin(0, *batches[k], None)), k
+            torch.cuda.synchronize()
