@@ -5,7 +5,7 @@
 //   norm    N = |grad_scale| sqrt(sum g^2), squares and sums in f64 (a square of an f32 is exact there: no overflow, no order to care
 //           about); coef = min(1, max_norm / (N + 1e-6)); N inf or NaN, or the range guard's verdict: the step is skipped
 //   AdamW   h = g * grad_scale * coef;  m += (h - m)(1 - b1);  v = v b2 + h^2 (1 - b2);
-//           p = p (1 - lr wd) - lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps)
+//           p = p (1 - lr wd) - lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps)      (the root times a rounded 1 / sqrt(1 - b2^t))
 //   8 bits  blocks of 128 consecutive elements of a tensor: x = q s, q in e4m3, s = 2^(max(E, -100) - 7), E = floor(log2 max |x|): a
 //           power of two scales without rounding and leaves the grid where it is while the block's largest value stays in its binade -
 //           an unchanged x keeps its code.  The state of v is its root u = sqrt(v): the 2^17 that a block spans are 2^34 in v.
